@@ -13,6 +13,7 @@ from .model.bilinear import Bilinear, BilinearUnit, heavy_linear, load  # noqa: 
 from .graph import CapturedTrainStep  # noqa: F401
 from .optim import Adam, clip_grad_norm_  # noqa: F401
 from .loss_log import LossRing  # noqa: F401
+from .row_ops import Dropout, LayerNorm, ResidualNorm, dropout, layer_norm, residual_norm  # noqa: F401
 from . import config  # noqa: F401
 
 
@@ -33,4 +34,5 @@ def configure_for_small_batches(enabled=True):
 
 
 __all__ = ["configure_for_small_batches", "BilinearUnit", "Bilinear", "heavy_linear", "load", "Adam", "clip_grad_norm_",
-           "CapturedTrainStep", "LossRing", "config"]
+           "CapturedTrainStep", "LossRing", "config", "layer_norm", "dropout", "residual_norm", "LayerNorm", "Dropout",
+           "ResidualNorm"]

@@ -40,6 +40,11 @@ class StepState(Structure):
                 ("step_size", c_float), ("bc2_sqrt", c_float)]
 
 
+class RowDrop(Structure):
+    _fields_ = [("p", c_double), ("seed", c_uint64), ("step", c_uint64), ("row_offset", c_int64),
+                ("step_dev", c_void_p), ("step_used", c_void_p), ("layer", c_int32), ("reserved", c_int32)]
+
+
 GradReadyFn = ctypes.CFUNCTYPE(None, c_void_p, c_int64, c_int64)
 SyncFn = ctypes.CFUNCTYPE(None, c_void_p, c_void_p, c_int64, c_int32)
 
@@ -154,6 +159,19 @@ _SIGNATURES = {
     "blh_linear_fwd_stats": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_int64, c_int64, c_int64]),
     "blh_dropout_mask": (c_int, [c_void_p, POINTER(Dropout), c_int32, c_int64, c_int32, c_void_p]),
+    # operators on rows (csrc/row_norm.hip, row_dropout.hip)
+    "blh_row_dropout": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, POINTER(RowDrop), c_int64, c_int64, c_int32]),
+    "blh_layer_norm_forward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_double, c_void_p, c_void_p,
+                                       c_void_p, c_int64, c_int64, c_int32, c_int32]),
+    "blh_row_norm_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "blh_layer_norm_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 7
+                                + [c_int64, c_int64, c_int64, c_int32, c_int32]),
+    "blh_residual_norm_forward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_double,
+                                          POINTER(RowDrop), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                          c_int32, c_int32, c_int32]),
+    "blh_residual_norm_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                           c_void_p, c_void_p, POINTER(RowDrop)] + [c_void_p] * 5
+                                   + [c_int64, c_int64, c_int64, c_int32, c_int32, c_int32]),
     # collectives issued by the library (opt-in data-parallel path, csrc/comm.hip)
     "blh_rccl_version": (c_int, []),
     "blh_rccl_unique_id": (c_int, [c_void_p, c_int64]),

@@ -1,0 +1,71 @@
+// Dropout of rows with a mask that is regenerated, never stored.
+//
+//   y[i][j] = u(i, j) >= t ? s x[i][j] : 0,    t = floor(65536 p + 1/2),  s = 65536 / (65536 - t)
+//
+// u(i, j): 16 bits of Philox4x32-10, one call for 8 columns of one GLOBAL row (row_offset + i):
+//   counter (row lo, j / 8 | row hi << 21, layer | 2^31, step lo), key (seed lo ^ step hi, seed hi),
+//   element e = j % 8 takes the half e & 1 of word e / 2.
+// The mask depends on (seed, step, layer, global row, column) alone: not on the type, the launch or how rows are spread
+// over devices.  p is rounded to a multiple of 2^-16 and s is the exact inverse of the rounded keep probability, so the
+// expectation of y is x.  The backward pass is the same map on dy: there is nothing to save.
+#include "row_ops.h"
+#include "row_ops_dev.h"
+
+namespace blh {
+
+int row_make_drop(const blh_row_drop* d, int64_t rows, RowDrop* out) {
+  if (!(d->p >= 0.0 && d->p <= 1.0) || d->layer < 0 || d->row_offset < 0) return BLH_ERR_INVALID_ARGUMENT;
+  if (d->row_offset > ROW_MAX_ROWS - rows) return BLH_ERR_SHAPE;
+  const uint32_t t = (uint32_t)(d->p * 65536.0 + 0.5);
+  *out = RowDrop{d->seed, d->step, d->step_dev, d->step_used, d->row_offset, (uint32_t)d->layer | 0x80000000u, t,
+                 t < 65536u ? (float)(65536.0 / (double)(65536u - t)) : 0.f};
+  return BLH_OK;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void row_dropout_kernel(const T* x, int64_t ldx, T* y, RowDrop drop, int64_t rows,
+                                                          int64_t width, int64_t units) {
+  const RowKey key = row_key(drop);
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * units; i += gridDim.x * 256ll) {
+    const int64_t row = i / units, unit = i - row * units, col = unit * ROW_UNIT;
+    float f[ROW_UNIT];
+    load_unit(x + row * ldx + col, width - col, f);
+    drop_unit(key, drop, drop.row_offset + row, unit, f);
+    store_unit(y + row * width + col, width - col, f);
+  }
+}
+
+template <typename T>
+static int launch_row_dropout(hipStream_t s, const void* x, int64_t ldx, void* y, const RowDrop& drop, int64_t rows,
+                              int64_t width) {
+  const int64_t units = ceil_div(width, ROW_UNIT);
+  const int64_t blocks = std::min<int64_t>(ceil_div(rows * units, 256), 4096);
+  hipLaunchKernelGGL((row_dropout_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T*>(x), ldx,
+                     static_cast<T*>(y), drop, rows, width, units);
+  BLH_HIP_TRY(hipGetLastError());
+  return BLH_OK;
+}
+
+}  // namespace blh
+
+using namespace blh;
+
+extern "C" {
+
+int blh_row_dropout(void* stream, const void* x, int64_t ldx, void* y, const blh_row_drop* drop, int64_t rows,
+                    int64_t width, int32_t dtype) {
+  if (!drop || !row_dtype_ok(dtype) || ldx < 0) return BLH_ERR_INVALID_ARGUMENT;
+  BLH_TRY(row_check_shape(rows, width));
+  RowDrop d;
+  BLH_TRY(row_make_drop(drop, rows, &d));
+  if (rows == 0) return BLH_OK;
+  if (!x || !y || !row_aligned(x, dtype) || !row_aligned(y, dtype)) return BLH_ERR_INVALID_ARGUMENT;
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case BLH_F32: return launch_row_dropout<float>(s, x, ldx, y, d, rows, width);
+    case BLH_BF16: return launch_row_dropout<bf16_t>(s, x, ldx, y, d, rows, width);
+    default: return launch_row_dropout<f16_t>(s, x, ldx, y, d, rows, width);
+  }
+}
+
+}  // extern "C"

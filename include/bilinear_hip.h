@@ -43,7 +43,8 @@ extern "C" {
 /* 5 (round 6): blh_context_grid_barrier_timeouts, BLH_OPT_DEFER_SLABS and BLH_OPT_SMALL_STEP = 2 (the persistent
  * small-batch launches) were removed with the slower opt-in variants they served.
  * 6 (round 6): blh_comm_* / blh_rccl_* / blh_train_step_dp (collectives issued by the library) and BLH_ERR_COMM added;
- * nothing removed or changed.                                                                              */
+ * nothing removed or changed.  (The row operators — blh_layer_norm_*, blh_residual_norm_*, blh_row_* — came later
+ * under the same number: new names only, what version 6 had is as it was.)                                  */
 #define BLH_ABI_VERSION 6
 
 typedef enum {
@@ -486,6 +487,61 @@ int blh_heavy_backward(blh_context* ctx, void* stream, const float* d_out, const
                        void* workspace, int64_t workspace_bytes, float* d_weight, float* d_bias,
                        float* d_gamma, float* d_beta, float* d_in, int64_t batch,
                        int32_t in_features, int32_t out_features);
+
+/* ---- operators on rows: layer norm, dropout with a regenerated mask, residual norm -------------------------------
+ * The counterparts of a stage's BatchNorm1d and Dropout(0.5) (model/bilinear.py:7-13) that need no batch and no stored
+ * mask, for blocks a user builds beside the lifter.  A tensor is `rows` rows of `width` columns, row i of an INPUT at
+ * element i * ld (ld >= 0: rows of a wider tensor, or one row repeated with ld = 0), outputs dense.  Base pointers are
+ * aligned to their element only; any width from 1 to 2^24, any number of rows (0: nothing is read, weight gradients are
+ * zero).  Types: activations `dtype`; `param_dtype` (weight, bias and their gradients) and `stream_dtype` (the residual
+ * stream) are `dtype` or BLH_F32.  Sums, means and moments are fp32; every result is rounded once.  No atomics: results
+ * do not change from run to run.  Inputs and outputs must not overlap, except that blh_row_dropout may work in place
+ * (y == x, ldx == width).  A row that holds an infinity or NaN makes that row's results NaN and no other's.           */
+typedef enum { BLH_F32 = 0, BLH_BF16 = 1, BLH_F16 = 2 } blh_dtype;
+
+/* Dropout of rows.  Element (i, j) is kept when a 16-bit draw u(i, j) >= t = floor(65536 p + 1/2) and then scaled by
+ * 65536 / (65536 - t); else it is 0 whatever x holds.  u: Philox4x32-10, one call per 8 columns of a global row
+ * (csrc/row_dropout.hip gives the counter).  The mask depends on (seed, step, layer, row_offset + i, j) alone: the
+ * backward pass is the same call on dy.  It is not the mask of blh_dropout (one bit per element, p = 0.5).
+ * row_offset + rows <= 2^43.                                                                                         */
+typedef struct {
+  double p;                  /* 0 .. 1                                                                                */
+  uint64_t seed, step;
+  int64_t row_offset;        /* global index of local row 0 (data parallel), >= 0                                     */
+  const uint64_t* step_dev;  /* device, or NULL: added to `step` when the kernel runs, so that a replayed graph draws
+                                another mask each time                                                                */
+  uint64_t* step_used;       /* device, or NULL: receives step + *step_dev when anything can be dropped (t > 0), for a
+                                backward pass that runs after *step_dev has moved on                                  */
+  int32_t layer;             /* stream id, >= 0: calls that must not share a mask differ in it or in `step`           */
+  int32_t reserved;
+} blh_row_drop;
+int blh_row_dropout(void* stream, const void* x, int64_t ldx, void* y, const blh_row_drop* drop, int64_t rows,
+                    int64_t width, int32_t dtype);
+
+/* y = (x - mean) rstd weight + bias over each row; weight / bias may be NULL (1 / 0).  mean, rstd (both or neither):
+ * [rows], what the backward reads.  eps >= 0.                                                                        */
+int blh_layer_norm_forward(void* stream, const void* x, int64_t ldx, const void* weight, const void* bias, double eps,
+                           void* y, float* mean, float* rstd, int64_t rows, int64_t width, int32_t dtype,
+                           int32_t param_dtype);
+/* dx, dweight, dbias: each may be NULL (not computed).  `workspace` (blh_row_norm_workspace_bytes, 16-byte aligned) is
+ * needed for dweight / dbias; its contents mean nothing between calls.                                               */
+int64_t blh_row_norm_workspace_bytes(int64_t rows, int64_t width);
+int blh_layer_norm_backward(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
+                            const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                            void* workspace, int64_t workspace_bytes, int64_t rows, int64_t width, int32_t dtype,
+                            int32_t param_dtype);
+/* h = residual + dropout(x), rounded to the stream's type; y = layer norm of that h.  drop == NULL: no dropout.      */
+int blh_residual_norm_forward(void* stream, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                              const void* weight, const void* bias, double eps, const blh_row_drop* drop, void* y,
+                              void* h, float* mean, float* rstd, int64_t rows, int64_t width, int32_t dtype,
+                              int32_t stream_dtype, int32_t param_dtype);
+/* dresidual = dh + (gradient through the norm), dx = dropout(dresidual) from the unrounded value.  dh NULL: no gradient
+ * reaches h by itself.  drop: as in the forward (drop->step_used is not written).                                    */
+int blh_residual_norm_backward(void* stream, const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h,
+                               int64_t ldh, const void* weight, const float* mean, const float* rstd,
+                               const blh_row_drop* drop, void* dx, void* dresidual, void* dweight, void* dbias,
+                               void* workspace, int64_t workspace_bytes, int64_t rows, int64_t width, int32_t dtype,
+                               int32_t stream_dtype, int32_t param_dtype);
 
 /* ---- validation metric ----------------------------------------------------------------
  * valid_bilinear.py:53-70: pred/target [B, joints*3] are de-normalised with the train-set
