@@ -1,0 +1,513 @@
+// PyTorch side of the row operators: argument checks, output allocation and autograd nodes around the C entry points
+// blh_layer_norm_*, blh_row_dropout and blh_residual_norm_* (host code only; bilinear_amd/row_ops.py loads it).
+//
+// Why C++ and not ctypes as the lifter's path: these calls are short — at a few hundred rows the kernels take 5-10 us —
+// and autograd runs a backward node on its device thread, where a Python node starts with cold caches.  Measured with
+// ctypes and a Python autograd.Function: forward + backward of a 64 x 1024 layer norm 143 us, of which the kernels are
+// 15; without a gradient 12.6 us.
+#include <ATen/hip/HIPContext.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <optional>
+#include <tuple>
+
+#include "../../include/bilinear_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> Optional;
+
+// ---- checks ---------------------------------------------------------------------------------------------------------
+
+const char* name_of(at::ScalarType t) { return c10::toString(t); }
+
+int32_t code_of(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return BLH_F32;
+    case at::kBFloat16: return BLH_BF16;
+    default: return BLH_F16;
+  }
+}
+
+void check_rows(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), "bilinear_amd row operators run only on a HIP device (MI355X); ", what, " is on '", t.device(),
+              "' and there is no CPU/ATen fallback.");
+  const auto s = t.scalar_type();
+  TORCH_CHECK(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, what, " must be float32, bfloat16 or float16, got ",
+              name_of(s));
+  TORCH_CHECK(t.layout() == at::kStrided, what, " must be a dense (strided) tensor");
+  TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, what, " needs a last axis of at least one column, got shape ", t.sizes());
+}
+
+void check_like(const Tensor& t, const Tensor& x, const char* what, bool or_float) {
+  TORCH_CHECK(t.device() == x.device(), what, " is on '", t.device(), "' where '", x.device(), "' is expected");
+  TORCH_CHECK(t.sizes() == x.sizes(), what, " has shape ", t.sizes(), " where ", x.sizes(), " is expected");
+  TORCH_CHECK(t.scalar_type() == x.scalar_type() || (or_float && t.scalar_type() == at::kFloat), what, " is ",
+              name_of(t.scalar_type()), " where ", name_of(x.scalar_type()), or_float ? " or Float" : "", " is expected");
+}
+
+void check_param(const Tensor& x, const Optional& t, const char* what) {
+  if (!t) return;
+  TORCH_CHECK(t->device() == x.device(), what, " is on '", t->device(), "' where '", x.device(), "' is expected");
+  TORCH_CHECK(t->dim() == 1 && t->size(0) == x.size(-1), what, " has shape ", t->sizes(), " where [", x.size(-1),
+              "] is expected");
+  TORCH_CHECK(t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat, what, " is ",
+              name_of(t->scalar_type()), " where Float or ", name_of(x.scalar_type()), " is expected");
+}
+
+// the type of weight and bias (fp32 where neither is given)
+int32_t check_params(const Tensor& x, const Optional& weight, const Optional& bias) {
+  check_param(x, weight, "weight");
+  check_param(x, bias, "bias");
+  TORCH_CHECK(!weight || !bias || weight->scalar_type() == bias->scalar_type(), "weight is ",
+              weight ? name_of(weight->scalar_type()) : "", " and bias ", bias ? name_of(bias->scalar_type()) : "",
+              ": one type for both is expected");
+  return weight ? code_of(weight->scalar_type()) : bias ? code_of(bias->scalar_type()) : BLH_F32;
+}
+
+void check_eps(double eps) { TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative, got ", eps); }
+
+struct Draws {
+  double p;
+  int64_t seed, step, layer, row_offset;
+  Tensor device_step;      // undefined: none
+};
+
+void check_draws(const Draws& d, const Tensor& x) {
+  TORCH_CHECK_VALUE(d.p >= 0.0 && d.p <= 1.0, "dropout probability has to be between 0 and 1, got ", d.p);
+  TORCH_CHECK_VALUE(d.seed >= 0 && d.step >= 0, "seed and step must be in [0, 2^63), got ", d.seed, " and ", d.step);
+  TORCH_CHECK_VALUE(d.layer >= 0 && d.layer < (int64_t(1) << 31), "layer must be in [0, 2^31), got ", d.layer);
+  TORCH_CHECK_VALUE(d.row_offset >= 0 && d.row_offset < (int64_t(1) << 43), "row_offset must be in [0, 2^43), got ",
+                    d.row_offset);
+  if (d.device_step.defined())
+    TORCH_CHECK(d.device_step.scalar_type() == at::kLong && d.device_step.numel() == 1 && d.device_step.device() == x.device(),
+                "device_step must be one int64 on '", x.device(), "'");
+}
+
+void check_status(int status, const char* what) {
+  if (status == BLH_OK) return;
+  TORCH_CHECK(false, "bilinear_amd: ", what, " failed: ", blh_status_string(status),
+              status == BLH_ERR_HIP ? " (hipError_t " + std::to_string(blh_last_hip_error()) + ")" : std::string());
+}
+
+// ---- native calls (checked tensors) ---------------------------------------------------------------------------------
+
+// Rows are read in place where the last axis is dense and the leading axes collapse to one, else from a dense copy.
+struct Rows {
+  Tensor t;
+  int64_t ld;
+  Rows() : ld(0) {}
+  explicit Rows(const Tensor& x) : t(x), ld(x.size(-1)) {
+    if (x.is_contiguous()) return;
+    const int64_t width = x.size(-1), n = x.dim();
+    if (x.stride(-1) == 1 || width == 1) {
+      // the step between consecutive rows, if all leading axes agree on one
+      int64_t step = -1, next = 0;
+      bool one = true;
+      for (int64_t a = n - 2; a >= 0 && one; --a) {
+        if (x.size(a) == 1) continue;
+        if (step < 0) step = x.stride(a); else one = x.stride(a) == next;
+        next = x.stride(a) * x.size(a);
+      }
+      if (one) {
+        ld = step < 0 ? width : step;
+        return;
+      }
+    }
+    t = x.contiguous();
+  }
+  const void* ptr() const { return t.defined() ? t.const_data_ptr() : nullptr; }
+};
+
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor plain(const Optional& t) { return t ? *t : Tensor(); }
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+void* stream_of(const Tensor& x) { return (void*)c10::hip::getCurrentHIPStream(x.get_device()).stream(); }
+int64_t rows_of(const Tensor& x) { return x.numel() / x.size(-1); }
+
+blh_row_drop drop_of(const Draws& d, const Tensor& used) {
+  return blh_row_drop{d.p, (uint64_t)d.seed, (uint64_t)d.step, d.row_offset,
+                      (const uint64_t*)ptr(d.device_step), (uint64_t*)out_ptr(used), (int32_t)d.layer, 0};
+}
+
+// what the backward reads of the forward, [rows] each (both NULL: not kept)
+struct Moments {
+  float* mean = nullptr;
+  float* rstd = nullptr;
+  Moments() {}
+  Moments(const Tensor& m, const Tensor& r) : mean(m.mutable_data_ptr<float>()), rstd(r.mutable_data_ptr<float>()) {}
+  explicit Moments(const Tensor& both) : mean(both.mutable_data_ptr<float>()), rstd(mean + both.size(1)) {}   // [2, rows]
+};
+
+Tensor both_moments(const Tensor& x) { return at::empty({2, rows_of(x)}, x.options().dtype(at::kFloat)); }
+
+Tensor used_step(const Draws& d) {
+  return d.device_step.defined() ? at::empty({1}, d.device_step.options()) : Tensor();
+}
+
+Tensor layer_norm_launch(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, int32_t param_code,
+                         Moments m) {
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Rows in(x);
+  Tensor y = at::empty(x.sizes(), x.options());
+  check_status(blh_layer_norm_forward(stream_of(x), in.ptr(), in.ld, ptr(weight), ptr(bias), eps, out_ptr(y), m.mean,
+                                      m.rstd, rows_of(x), x.size(-1), code_of(x.scalar_type()), param_code),
+               "blh_layer_norm_forward");
+  return y;
+}
+
+struct ParamGrads {
+  Tensor weight, bias, workspace;
+  ParamGrads(const Tensor& x, bool need_weight, bool need_bias, int32_t code) {
+    const auto o = x.options().dtype(code == BLH_F32 ? at::kFloat : x.scalar_type());
+    if (need_weight) weight = at::empty({x.size(-1)}, o);
+    if (need_bias) bias = at::empty({x.size(-1)}, o);
+    if (need_weight || need_bias) {
+      const int64_t need = blh_row_norm_workspace_bytes(rows_of(x), x.size(-1));
+      if (need < 0) check_status((int)need, "blh_row_norm_workspace_bytes");
+      workspace = at::empty({need}, x.options().dtype(at::kByte));
+    }
+  }
+  int64_t bytes() const { return workspace.defined() ? workspace.numel() : 0; }
+};
+
+variable_list layer_norm_backward_launch(const Tensor& dy, const Tensor& x, const Tensor& weight, Moments m,
+                                         bool need_x, bool need_weight, bool need_bias, int32_t code) {
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Rows gy(dy), in(x);
+  Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : Tensor();
+  const ParamGrads g(x, need_weight, need_bias, code);
+  check_status(blh_layer_norm_backward(stream_of(x), gy.ptr(), gy.ld, in.ptr(), in.ld, ptr(weight), m.mean, m.rstd,
+                                       out_ptr(dx), out_ptr(g.weight), out_ptr(g.bias), out_ptr(g.workspace), g.bytes(),
+                                       rows_of(x), x.size(-1), code_of(x.scalar_type()), code),
+               "blh_layer_norm_backward");
+  return {dx, g.weight, g.bias};
+}
+
+Tensor dropout_launch(const Tensor& x, const Draws& d, const Tensor& used) {
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Rows in(x);
+  Tensor y = at::empty(x.sizes(), x.options());
+  const blh_row_drop drop = drop_of(d, used);
+  check_status(blh_row_dropout(stream_of(x), in.ptr(), in.ld, out_ptr(y), &drop, rows_of(x), x.size(-1),
+                               code_of(x.scalar_type())), "blh_row_dropout");
+  return y;
+}
+
+std::tuple<Tensor, Tensor> residual_norm_launch(const Tensor& x, const Tensor& residual, const Tensor& weight,
+                                                const Tensor& bias, double eps, const Draws& d, int32_t param_code,
+                                                Moments m, const Tensor& used) {
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Rows in(x), res(residual);
+  Tensor y = at::empty(x.sizes(), x.options());
+  Tensor h = at::empty(x.sizes(), residual.options());
+  const blh_row_drop drop = drop_of(d, used);
+  check_status(blh_residual_norm_forward(stream_of(x), in.ptr(), in.ld, res.ptr(), res.ld, ptr(weight), ptr(bias), eps,
+                                         d.p > 0.0 ? &drop : nullptr, out_ptr(y), out_ptr(h), m.mean, m.rstd,
+                                         rows_of(x), x.size(-1), code_of(x.scalar_type()),
+                                         code_of(residual.scalar_type()), param_code), "blh_residual_norm_forward");
+  return {y, h};
+}
+
+// {dx, dresidual, dweight, dbias}
+variable_list residual_norm_backward_launch(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& weight,
+                                            Moments m, const Draws& d, bool need_x,
+                                            bool need_residual, bool need_weight, bool need_bias, int32_t code) {
+  const c10::OptionalDeviceGuard guard(h.device());
+  const Rows gy(dy), in(h), gh = dh.defined() ? Rows(dh) : Rows();
+  Tensor dx = need_x ? at::empty(h.sizes(), dy.options()) : Tensor();
+  Tensor dres = need_residual ? at::empty(h.sizes(), h.options()) : Tensor();
+  const ParamGrads g(dy, need_weight, need_bias, code);
+  const blh_row_drop drop = drop_of(d, Tensor());
+  check_status(blh_residual_norm_backward(stream_of(h), gy.ptr(), gy.ld, gh.ptr(), gh.ld, in.ptr(), in.ld, ptr(weight),
+                                          m.mean, m.rstd, d.p > 0.0 ? &drop : nullptr, out_ptr(dx), out_ptr(dres),
+                                          out_ptr(g.weight), out_ptr(g.bias), out_ptr(g.workspace), g.bytes(), rows_of(h),
+                                          h.size(-1), code_of(dy.scalar_type()), code_of(h.scalar_type()), code),
+               "blh_residual_norm_backward");
+  return {dx, dres, g.weight, g.bias};
+}
+
+// ---- autograd -------------------------------------------------------------------------------------------------------
+
+// A leaf's gradient accumulator belongs to the stream it was made on.  One that an eager graph on the DEFAULT stream still
+// holds cannot take part in a stream capture (that stream cannot be captured: the capture would break inside the autograd
+// engine, where the error ends the process), so such a call is refused before anything is enqueued.
+void refuse_eager_leaves(std::initializer_list<const Tensor*> inputs) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) continue;
+    const auto s = node->stream();
+    TORCH_CHECK(!s || s->id() != 0,
+                "bilinear_amd: a tensor that needs a gradient in this stream capture is still part of an eager autograd "
+                "graph recorded on the default stream.  Drop that graph (its outputs and losses) before the capture, or "
+                "run the eager steps on a side stream (torch.cuda.stream).");
+  }
+}
+
+// The formulas below are not themselves differentiable: a backward pass through them is refused where it is asked for.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "bilinear_amd row operators: trying to differentiate the backward pass, which is not supported", (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+struct LayerNormBackward : public torch::autograd::Node {
+  SavedVariable x, weight;
+  Tensor moments;           // mean and rstd, [2, rows]
+  int32_t code = 0;
+  std::string name() const override { return "BilinearLayerNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data();
+    weight.reset_data();
+    moments.reset();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return variable_list(3);
+    const Tensor in = x.unpack(), w = dense(weight.unpack());
+    return once(layer_norm_backward_launch(grads[0], in, w, Moments(moments), task_should_compute_output(0),
+                                           task_should_compute_output(1), task_should_compute_output(2), code));
+  }
+};
+
+struct RowDropoutBackward : public torch::autograd::Node {
+  Draws d;
+  std::string name() const override { return "BilinearRowDropoutBackward"; }
+  variable_list apply(variable_list&& grads) override {
+    if (!grads[0].defined()) return variable_list(1);
+    return once({dropout_launch(grads[0], d, Tensor())});
+  }
+};
+
+struct ResidualNormBackward : public torch::autograd::Node {
+  SavedVariable h, weight;
+  Tensor moments;
+  Draws d;
+  int32_t code = 0;
+  at::ScalarType dtype = at::kFloat;
+  std::string name() const override { return "BilinearResidualNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    h.reset_data();
+    weight.reset_data();
+    moments.reset();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined() && !grads[1].defined()) return variable_list(4);
+    const Tensor stream = h.unpack(shared_from_this()), w = dense(weight.unpack());
+    // only the stream went on: the norm's share is zero
+    const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(stream.sizes(), stream.options().dtype(dtype));
+    const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1);
+    // without dropout and with one type both branches of the sum get the same gradient: it is written once
+    const bool same = need_x && need_r && stream.scalar_type() == dtype && (int64_t)(d.p * 65536.0 + 0.5) == 0;
+    variable_list out = residual_norm_backward_launch(dy, grads[1], stream, w, Moments(moments), d, need_x && !same,
+                                                      need_r, task_should_compute_output(2),
+                                                      task_should_compute_output(3), code);
+    if (same) out[0] = out[1];
+    return once(std::move(out));
+  }
+};
+
+template <typename N> std::shared_ptr<N> make_node() {
+  return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
+}
+
+bool wants_grad(std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// ---- what Python calls ----------------------------------------------------------------------------------------------
+
+Tensor layer_norm(const Tensor& x, const Optional& weight, const Optional& bias, double eps) {
+  check_rows(x, "x");
+  const int32_t code = check_params(x, weight, bias);
+  check_eps(eps);
+  const Tensor w = plain(weight), b = plain(bias);
+  if (!wants_grad({&x, &w, &b})) return layer_norm_launch(x, dense(w), dense(b), eps, code, Moments());
+  refuse_eager_leaves({&x, &w, &b});
+  const Tensor both = both_moments(x);
+  Tensor y = layer_norm_launch(x, dense(w), dense(b), eps, code, Moments(both));
+  auto node = make_node<LayerNormBackward>();
+  node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+  node->x = SavedVariable(x, false);
+  node->weight = SavedVariable(w, false);
+  node->moments = both;
+  node->code = code;
+  torch::autograd::set_history(y, node);
+  return y;
+}
+
+Tensor dropout(const Tensor& x, double p, int64_t seed, int64_t step, int64_t layer, int64_t row_offset,
+               const Optional& device_step) {
+  check_rows(x, "x");
+  Draws d{p, seed, step, layer, row_offset, plain(device_step)};
+  check_draws(d, x);
+  const bool grad = wants_grad({&x});
+  if (grad) refuse_eager_leaves({&x});
+  const Tensor used = grad ? used_step(d) : Tensor();
+  Tensor y = dropout_launch(x, d, used);
+  if (grad) {
+    if (used.defined()) d.step = 0;
+    d.device_step = used;
+    auto node = make_node<RowDropoutBackward>();
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->d = d;
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
+std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& residual, const Optional& weight,
+                                         const Optional& bias, double eps, double p, int64_t seed, int64_t step,
+                                         int64_t layer, int64_t row_offset, const Optional& device_step) {
+  check_rows(x, "x");
+  check_like(residual, x, "residual", true);
+  const int32_t code = check_params(x, weight, bias);
+  check_eps(eps);
+  Draws d{p, seed, step, layer, row_offset, plain(device_step)};
+  check_draws(d, x);
+  const Tensor w = plain(weight), b = plain(bias);
+  const bool grad = wants_grad({&x, &residual, &w, &b});
+  if (!grad) return residual_norm_launch(x, residual, dense(w), dense(b), eps, d, code, Moments(), Tensor());
+  refuse_eager_leaves({&x, &residual, &w, &b});
+  const Tensor both = both_moments(x);
+  const Tensor used = used_step(d);
+  auto [y, h] = residual_norm_launch(x, residual, dense(w), dense(b), eps, d, code, Moments(both), used);
+  if (used.defined()) d.step = 0;
+  d.device_step = used;
+  auto node = make_node<ResidualNormBackward>();
+  node->set_next_edges(torch::autograd::collect_next_edges(x, residual, w, b));
+  node->weight = SavedVariable(w, false);
+  node->moments = both;
+  node->d = d;
+  node->code = code;
+  node->dtype = x.scalar_type();
+  torch::autograd::set_history({y, h}, node);
+  node->h = SavedVariable(h, true);
+  return {y, h};
+}
+
+// The custom operators' implementations: plain functions, outputs that were not asked for come back empty.
+
+Tensor filled(const Tensor& t, const Tensor& x, at::ScalarType s) {
+  return t.defined() ? t : at::empty({0}, x.options().dtype(s));
+}
+
+void check_stats(const Tensor& x, const Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == rows_of(x) && t.is_contiguous() && t.device() == x.device(), what,
+              " must be ", rows_of(x), " dense float32 values on '", x.device(), "'");
+}
+
+int32_t check_code(const Tensor& x, const Optional& weight, int64_t code) {
+  TORCH_CHECK(code == BLH_F32 || code == code_of(x.scalar_type()), "param_code must be 0 (float32) or that of ",
+              name_of(x.scalar_type()));
+  TORCH_CHECK(!weight || code_of(weight->scalar_type()) == code, "param_code is not the weight's type");
+  return (int32_t)code;
+}
+
+std::tuple<Tensor, Tensor, Tensor> op_layer_norm(const Tensor& x, const Optional& weight, const Optional& bias, double eps) {
+  check_rows(x, "x");
+  const int32_t code = check_params(x, weight, bias);
+  check_eps(eps);
+  const auto o = x.options().dtype(at::kFloat);
+  const Tensor mean = at::empty({rows_of(x)}, o), rstd = at::empty({rows_of(x)}, o);
+  Tensor y = layer_norm_launch(x, dense(plain(weight)), dense(plain(bias)), eps, code, Moments(mean, rstd));
+  return {y, mean, rstd};
+}
+
+std::tuple<Tensor, Tensor, Tensor> op_layer_norm_backward(const Tensor& dy, const Tensor& x, const Optional& weight,
+                                                          const Tensor& mean, const Tensor& rstd, bool need_x,
+                                                          bool need_weight, bool need_bias, int64_t param_code) {
+  check_rows(x, "x");
+  check_like(dy, x, "dy", false);
+  check_param(x, weight, "weight");
+  check_stats(x, mean, "mean");
+  check_stats(x, rstd, "rstd");
+  const int32_t code = check_code(x, weight, param_code);
+  const auto g = layer_norm_backward_launch(dy, x, dense(plain(weight)), Moments(mean, rstd), need_x, need_weight,
+                                            need_bias, code);
+  const auto s = code == BLH_F32 ? at::kFloat : x.scalar_type();
+  return {filled(g[0], x, x.scalar_type()), filled(g[1], x, s), filled(g[2], x, s)};
+}
+
+std::tuple<Tensor, Tensor> op_row_dropout(const Tensor& x, double p, int64_t seed, int64_t step, int64_t layer,
+                                          int64_t row_offset, const Optional& device_step) {
+  check_rows(x, "x");
+  const Draws d{p, seed, step, layer, row_offset, plain(device_step)};
+  check_draws(d, x);
+  const Tensor used = used_step(d);
+  Tensor y = dropout_launch(x, d, used);
+  return {y, filled(used, x, at::kLong)};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> op_residual_norm(
+    const Tensor& x, const Tensor& residual, const Optional& weight, const Optional& bias, double eps, double p,
+    int64_t seed, int64_t step, int64_t layer, int64_t row_offset, const Optional& device_step) {
+  check_rows(x, "x");
+  check_like(residual, x, "residual", true);
+  const int32_t code = check_params(x, weight, bias);
+  check_eps(eps);
+  const Draws d{p, seed, step, layer, row_offset, plain(device_step)};
+  check_draws(d, x);
+  const auto o = x.options().dtype(at::kFloat);
+  const Tensor mean = at::empty({rows_of(x)}, o), rstd = at::empty({rows_of(x)}, o);
+  const Tensor used = used_step(d);
+  auto [y, h] = residual_norm_launch(x, residual, dense(plain(weight)), dense(plain(bias)), eps, d, code,
+                                     Moments(mean, rstd), used);
+  return {y, h, mean, rstd, filled(used, x, at::kLong)};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> op_residual_norm_backward(
+    const Tensor& dy, const Optional& dh, const Tensor& h, const Optional& weight, const Tensor& mean, const Tensor& rstd,
+    double p, int64_t seed, int64_t step, int64_t layer, int64_t row_offset, const Optional& device_step, bool need_x,
+    bool need_residual, bool need_weight, bool need_bias, int64_t param_code) {
+  check_rows(dy, "dy");
+  check_like(h, dy, "h", true);
+  if (dh) check_like(*dh, h, "dh", false);
+  check_param(dy, weight, "weight");
+  check_stats(h, mean, "mean");
+  check_stats(h, rstd, "rstd");
+  const int32_t code = check_code(dy, weight, param_code);
+  const Draws d{p, seed, step, layer, row_offset, plain(device_step)};
+  check_draws(d, dy);
+  const auto g = residual_norm_backward_launch(dy, plain(dh), h, dense(plain(weight)), Moments(mean, rstd), d, need_x, need_residual, need_weight, need_bias,
+                                               code);
+  const auto s = code == BLH_F32 ? at::kFloat : dy.scalar_type();
+  return {filled(g[0], dy, dy.scalar_type()), filled(g[1], h, h.scalar_type()), filled(g[2], dy, s), filled(g[3], dy, s)};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_rows, m) {
+  const auto release = pybind11::call_guard<pybind11::gil_scoped_release>();
+  m.def("layer_norm", &layer_norm, release);
+  m.def("dropout", &dropout, release);
+  m.def("residual_norm", &residual_norm, release);
+  m.def("op_layer_norm", &op_layer_norm, release);
+  m.def("op_layer_norm_backward", &op_layer_norm_backward, release);
+  m.def("op_row_dropout", &op_row_dropout, release);
+  m.def("op_residual_norm", &op_residual_norm, release);
+  m.def("op_residual_norm_backward", &op_residual_norm_backward, release);
+}

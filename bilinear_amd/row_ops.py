@@ -17,7 +17,9 @@ must live on a HIP device: there is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
+import importlib.machinery
+import importlib.util
+import os
 
 import torch
 import torch.nn as nn
@@ -28,199 +30,29 @@ from .ops import _LIB
 __all__ = ["layer_norm", "dropout", "residual_norm", "LayerNorm", "Dropout", "ResidualNorm"]
 
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # blh_dtype
-_LIMIT63 = 1 << 63
+_BINDING = os.path.join(os.path.dirname(N.LIB_PATH), "_rows.so")
+_rows = None
 
 
-# ---- checks ---------------------------------------------------------------------------------------------------------
-
-def _check_rows(t, what):
-    if t.device.type != "cuda":
-        raise RuntimeError("bilinear_amd row operators run only on a HIP device (MI355X); %s is on '%s' and there is no "
-                           "CPU/ATen fallback." % (what, t.device))
-    if t.dtype not in _CODES:
-        raise RuntimeError("%s must be float32, bfloat16 or float16, got %s" % (what, t.dtype))
-    if t.dim() < 1 or t.shape[-1] < 1:
-        raise RuntimeError("%s needs a last axis of at least one column, got shape %s" % (what, tuple(t.shape)))
-
-
-def _check_like(t, x, what, dtypes):
-    if t.device != x.device:
-        raise RuntimeError("%s is on '%s' where '%s' is expected" % (what, t.device, x.device))
-    if t.shape != x.shape:
-        raise RuntimeError("%s has shape %s where %s is expected" % (what, tuple(t.shape), tuple(x.shape)))
-    if t.dtype not in dtypes:
-        raise RuntimeError("%s is %s where %s is expected" % (what, t.dtype, " or ".join(str(d) for d in dtypes)))
-
-
-def _check_params(x, weight, bias):
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        if t.device != x.device:
-            raise RuntimeError("%s is on '%s' where '%s' is expected" % (what, t.device, x.device))
-        if t.dim() != 1 or t.shape[0] != x.shape[-1]:
-            raise RuntimeError("%s has shape %s where (%d,) is expected" % (what, tuple(t.shape), x.shape[-1]))
-        if t.dtype != x.dtype and t.dtype != torch.float32:
-            raise RuntimeError("%s is %s where float32 or %s is expected" % (what, t.dtype, x.dtype))
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise RuntimeError("weight is %s and bias %s: one type for both is expected" % (weight.dtype, bias.dtype))
-
-
-def _check_eps(eps):
-    if not eps >= 0.0:
-        raise ValueError("eps must not be negative, got %r" % (eps,))
-
-
-def _check_draws(p, seed, step, layer, row_offset, device_step, x):
-    if not 0.0 <= p <= 1.0:
-        raise ValueError("dropout probability has to be between 0 and 1, got %r" % (p,))
-    for v, what in ((seed, "seed"), (step, "step")):
-        if not 0 <= v < _LIMIT63:
-            raise ValueError("%s must be in [0, 2^63), got %r" % (what, v))
-    if not 0 <= layer < 1 << 31:
-        raise ValueError("layer must be in [0, 2^31), got %r" % (layer,))
-    if not 0 <= row_offset < 1 << 43:
-        raise ValueError("row_offset must be in [0, 2^43), got %r" % (row_offset,))
-    if device_step is not None and (device_step.dtype != torch.int64 or device_step.numel() != 1
-                                    or device_step.device != x.device):
-        raise RuntimeError("device_step must be one int64 on '%s'" % (x.device,))
-
-
-# ---- native calls (tensors are checked; impls of the custom operators) -----------------------------------------------
-
-def _rows(t):
-    """(tensor to read, elements between its rows): rows are read in place where the last axis is dense and the leading
-    axes collapse to one, else from a dense copy."""
-    width = t.shape[-1]
-    if t.is_contiguous():
-        return t, width
-    if t.stride(-1) == 1 or width == 1:
-        if t.dim() == 2:
-            return t, t.stride(0)
-        try:
-            v = t.view(-1, width)
-            return v, v.stride(0)
-        except RuntimeError:
-            pass
-    return t.contiguous(), width
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _dense(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
-
-
-def _launch(name, x, *args):
-    """One entry point on the current stream of x's device (which need not be the current device)."""
-    index = x.get_device()
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return _launch(name, x, *args)
-    status = getattr(N.lib(), name)(torch._C._cuda_getCurrentRawStream(index), *args)
-    if status:
-        N.check(status, name)
-
-
-def _drop(p, seed, step, layer, row_offset, device_step, used):
-    return ctypes.byref(N.RowDrop(p, seed, step, row_offset, _ptr(device_step), _ptr(used), layer, 0))
+def _native():
+    """The PyTorch side of the operators (csrc/torch_rows.cpp: argument checks, allocation, autograd nodes), loaded once.
+    There is no other implementation: a missing library raises."""
+    global _rows
+    if _rows is None:
+        N.lib()                       # libbilinear_hip.so against the HIP runtime torch has loaded
+        if not os.path.exists(_BINDING):
+            raise RuntimeError("bilinear_amd: %s not found. Build it with `python -c 'import __graft_entry__ as g; "
+                               "g.build()'` or `make -C bilinear_amd/csrc`. There is no fallback path." % _BINDING)
+        loader = importlib.machinery.ExtensionFileLoader("_rows", _BINDING)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_rows", loader))
+        loader.exec_module(module)
+        _rows = module
+    return _rows
 
 
 def _param_code(x, weight, bias):
     t = weight if weight is not None else bias
     return 0 if t is None else _CODES[t.dtype]
-
-
-def _workspace(x, rows, width):
-    need = N.lib().blh_row_norm_workspace_bytes(rows, width)
-    if need < 0:
-        N.check(int(need), "blh_row_norm_workspace_bytes")
-    return torch.empty(need, dtype=torch.uint8, device=x.device), need
-
-
-def _layer_norm(x, weight, bias, eps, save=True):
-    width = x.shape[-1]
-    rows = x.numel() // width
-    src, ld = _rows(x)
-    weight, bias = _dense(weight), _dense(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows) if save else (2, 0), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    _launch("blh_layer_norm_forward", x, src.data_ptr(), ld, _ptr(weight), _ptr(bias), eps, y.data_ptr(),
-            mean.data_ptr() if save else None, rstd.data_ptr() if save else None, rows, width, _CODES[x.dtype],
-            _param_code(x, weight, bias))
-    return y, mean, rstd
-
-
-def _grads_of_params(x, width, need_weight, need_bias, code):
-    dtype = torch.float32 if code == 0 else x.dtype
-    dw = torch.empty(width if need_weight else 0, dtype=dtype, device=x.device)
-    db = torch.empty(width if need_bias else 0, dtype=dtype, device=x.device)
-    return dw, db
-
-
-def _layer_norm_backward(dy, x, weight, mean, rstd, need_x, need_weight, need_bias, param_code):
-    width = x.shape[-1]
-    rows = x.numel() // width
-    (dy_, lddy), (x_, ldx) = _rows(dy), _rows(x)
-    weight = _dense(weight)
-    dx = torch.empty(x.shape if need_x else (0,), dtype=x.dtype, device=x.device)
-    dw, db = _grads_of_params(x, width, need_weight, need_bias, param_code)
-    ws, size = _workspace(x, rows, width) if need_weight or need_bias else (None, 0)
-    _launch("blh_layer_norm_backward", x, dy_.data_ptr(), lddy, x_.data_ptr(), ldx, _ptr(weight), mean.data_ptr(),
-            rstd.data_ptr(), dx.data_ptr() if need_x else None, dw.data_ptr() if need_weight else None,
-            db.data_ptr() if need_bias else None, _ptr(ws), size, rows, width, _CODES[x.dtype], param_code)
-    return dx, dw, db
-
-
-def _row_dropout(x, p, seed, step, layer, row_offset, device_step):
-    width = x.shape[-1]
-    src, ld = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    used = torch.empty(0 if device_step is None else 1, dtype=torch.int64, device=x.device)
-    _launch("blh_row_dropout", x, src.data_ptr(), ld, y.data_ptr(),
-            _drop(p, seed, step, layer, row_offset, device_step, None if device_step is None else used),
-            x.numel() // width, width, _CODES[x.dtype])
-    return y, used
-
-
-def _residual_norm(x, residual, weight, bias, eps, p, seed, step, layer, row_offset, device_step, save=True):
-    width = x.shape[-1]
-    rows = x.numel() // width
-    (src, ldx), (res, ldr) = _rows(x), _rows(residual)
-    weight, bias = _dense(weight), _dense(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    stats = torch.empty((2, rows) if save else (2, 0), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    used = torch.empty(0 if device_step is None else 1, dtype=torch.int64, device=x.device)
-    drop = _drop(p, seed, step, layer, row_offset, device_step, None if device_step is None else used) if p else None
-    _launch("blh_residual_norm_forward", x, src.data_ptr(), ldx, res.data_ptr(), ldr, _ptr(weight), _ptr(bias), eps, drop,
-            y.data_ptr(), h.data_ptr(), mean.data_ptr() if save else None, rstd.data_ptr() if save else None, rows, width,
-            _CODES[x.dtype], _CODES[residual.dtype], _param_code(x, weight, bias))
-    return y, h, mean, rstd, used
-
-
-def _residual_norm_backward(dy, dh, h, weight, mean, rstd, p, seed, step, layer, row_offset, device_step, need_x,
-                            need_residual, need_weight, need_bias, param_code):
-    width = h.shape[-1]
-    rows = h.numel() // width
-    (dy_, lddy), (h_, ldh) = _rows(dy), _rows(h)
-    dh_, lddh = (None, 0) if dh is None else _rows(dh)
-    weight = _dense(weight)
-    dx = torch.empty(h.shape if need_x else (0,), dtype=dy.dtype, device=h.device)
-    dres = torch.empty(h.shape if need_residual else (0,), dtype=h.dtype, device=h.device)
-    dw, db = _grads_of_params(dy, width, need_weight, need_bias, param_code)
-    ws, size = _workspace(h, rows, width) if need_weight or need_bias else (None, 0)
-    drop = _drop(p, seed, step, layer, row_offset, device_step, None) if p else None
-    _launch("blh_residual_norm_backward", h, dy_.data_ptr(), lddy, _ptr(dh_), lddh, h_.data_ptr(), ldh, _ptr(weight),
-            mean.data_ptr(), rstd.data_ptr(), drop, dx.data_ptr() if need_x else None,
-            dres.data_ptr() if need_residual else None, dw.data_ptr() if need_weight else None,
-            db.data_ptr() if need_bias else None, _ptr(ws), size, rows, width, _CODES[dy.dtype], _CODES[h.dtype],
-            param_code)
-    return dx, dres, dw, db
 
 
 # ---- custom operators -----------------------------------------------------------------------------------------------
@@ -238,71 +70,8 @@ _LIB.define("residual_norm_backward(Tensor dy, Tensor? dh, Tensor h, Tensor? wei
             "-> (Tensor, Tensor, Tensor, Tensor)" % _DRAWS)
 
 
-def _op_layer_norm(x, weight, bias, eps):
-    _check_rows(x, "x")
-    _check_params(x, weight, bias)
-    _check_eps(eps)
-    return _layer_norm(x, weight, bias, eps)
-
-
-def _check_stats(x, mean, rstd):
-    rows = x.numel() // x.shape[-1]
-    for t, what in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous() or t.device != x.device:
-            raise RuntimeError("%s must be %d dense float32 values on '%s'" % (what, rows, x.device))
-
-
-def _check_param_code(x, code):
-    if code not in (0, _CODES[x.dtype]):
-        raise RuntimeError("param_code must be 0 (float32) or %d (%s)" % (_CODES[x.dtype], x.dtype))
-
-
-def _op_layer_norm_backward(dy, x, weight, mean, rstd, need_x, need_weight, need_bias, param_code):
-    _check_rows(x, "x")
-    _check_like(dy, x, "dy", (x.dtype,))
-    _check_params(x, weight, None)
-    _check_stats(x, mean, rstd)
-    _check_param_code(x, param_code)
-    if weight is not None and _CODES[weight.dtype] != param_code:
-        raise RuntimeError("param_code is not the weight's type")
-    return _layer_norm_backward(dy, x, weight, mean, rstd, need_x, need_weight, need_bias, param_code)
-
-
-def _op_row_dropout(x, p, seed, step, layer, row_offset, device_step):
-    _check_rows(x, "x")
-    _check_draws(p, seed, step, layer, row_offset, device_step, x)
-    return _row_dropout(x, p, seed, step, layer, row_offset, device_step)
-
-
-def _op_residual_norm(x, residual, weight, bias, eps, p, seed, step, layer, row_offset, device_step):
-    _check_rows(x, "x")
-    _check_like(residual, x, "residual", (x.dtype, torch.float32))
-    _check_params(x, weight, bias)
-    _check_eps(eps)
-    _check_draws(p, seed, step, layer, row_offset, device_step, x)
-    return _residual_norm(x, residual, weight, bias, eps, p, seed, step, layer, row_offset, device_step)
-
-
-def _op_residual_norm_backward(dy, dh, h, weight, mean, rstd, p, seed, step, layer, row_offset, device_step, need_x,
-                               need_residual, need_weight, need_bias, param_code):
-    _check_rows(dy, "dy")
-    _check_like(h, dy, "h", (dy.dtype, torch.float32))
-    if dh is not None:
-        _check_like(dh, dy, "dh", (h.dtype,))
-    _check_params(dy, weight, None)
-    _check_stats(h, mean, rstd)
-    _check_param_code(dy, param_code)
-    if weight is not None and _CODES[weight.dtype] != param_code:
-        raise RuntimeError("param_code is not the weight's type")
-    _check_draws(p, seed, step, layer, row_offset, device_step, dy)
-    return _residual_norm_backward(dy, dh, h, weight, mean, rstd, p, seed, step, layer, row_offset, device_step, need_x,
-                                   need_residual, need_weight, need_bias, param_code)
-
-
-for _name, _impl in (("layer_norm", _op_layer_norm), ("layer_norm_backward", _op_layer_norm_backward),
-                     ("row_dropout", _op_row_dropout), ("residual_norm", _op_residual_norm),
-                     ("residual_norm_backward", _op_residual_norm_backward)):
-    _LIB.impl(_name, _impl, "CUDA")
+for _name in ("layer_norm", "layer_norm_backward", "row_dropout", "residual_norm", "residual_norm_backward"):
+    _LIB.impl(_name, lambda *args, _name="op_" + _name: getattr(_native(), _name)(*args), "CUDA")
 
 
 def _new(x, shape, dtype=None):
@@ -391,106 +160,6 @@ torch.library.register_autograd("bilinear_hip::row_dropout", _drop_formula, setu
 torch.library.register_autograd("bilinear_hip::residual_norm", _res_formula, setup_context=_res_setup, lib=_LIB)
 
 
-# ---- eager autograd bridges (the same native calls without the operator dispatch) ------------------------------------
-
-_once = torch.autograd.function.once_differentiable
-
-
-class _LayerNormFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _layer_norm(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.code = _param_code(x, weight, bias)
-        return y
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad[:3]
-        return _pick(need, _layer_norm_backward(dy, x, weight, mean, rstd, *need, ctx.code)) + (None,)
-
-
-class _DropoutFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, seed, step, layer, row_offset, device_step):
-        y, used = _row_dropout(x, p, seed, step, layer, row_offset, device_step)
-        ctx.used = None if device_step is None else used
-        ctx.draws = (p, seed, step if device_step is None else 0, layer, row_offset)
-        return y
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        return (_row_dropout(dy, *ctx.draws, ctx.used)[0],) + (None,) * 6
-
-
-class _ResidualNormFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps, p, seed, step, layer, row_offset, device_step):
-        y, h, mean, rstd, used = _residual_norm(x, residual, weight, bias, eps, p, seed, step, layer, row_offset,
-                                                device_step)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(h, weight, mean, rstd)
-        ctx.used = None if device_step is None else used
-        ctx.draws = (p, seed, step if device_step is None else 0, layer, row_offset)
-        ctx.code, ctx.dtype = _param_code(x, weight, bias), x.dtype
-        return y, h
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy, dh):
-        h, weight, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad[:4]
-        if dy is None and dh is None:
-            return (None,) * 11
-        if dy is None:               # only the stream went on: the norm's share is zero
-            dy = torch.zeros(h.shape, dtype=ctx.dtype, device=h.device)
-        # without dropout and with one type both branches of the sum get the same gradient: it is written once
-        same = need[0] and need[1] and h.dtype == ctx.dtype and int(ctx.draws[0] * 65536.0 + 0.5) == 0
-        dx, dres, dw, db = _residual_norm_backward(dy, dh, h, weight, mean, rstd, *ctx.draws, ctx.used,
-                                                   need[0] and not same, *need[1:], ctx.code)
-        return _pick(need, (dres if same else dx, dres, dw, db)) + (None,) * 7
-
-
-# A leaf's gradient accumulator belongs to the stream it was made on.  One that an eager graph on the DEFAULT stream still
-# holds cannot take part in a stream capture (the default stream cannot be captured: the capture would break inside the
-# autograd engine, where the error ends the process), so such calls are refused while a graph is being captured.
-_EAGER = "bilinear_hip_default_stream"
-
-
-def _capturing():
-    return torch._C._cuda_isCurrentStreamCapturing()
-
-
-def _refuse_eager_leaves(tensors):
-    for t in tensors:
-        if t is not None and t.requires_grad and t.is_leaf:
-            if torch.autograd.graph.get_gradient_edge(t).node.metadata.get(_EAGER):
-                raise RuntimeError(
-                    "bilinear_amd: a tensor that needs a gradient in this stream capture is still part of an eager autograd "
-                    "graph recorded on the default stream.  Drop that graph (its outputs and losses) before the capture, or "
-                    "run the eager steps on a side stream (torch.cuda.stream).")
-
-
-def _apply(function, leaves, *args):
-    if _capturing():
-        _refuse_eager_leaves(leaves)
-        return function.apply(*args)
-    out = function.apply(*args)
-    first = out[0] if type(out) is tuple else out
-    if first.grad_fn is not None and not torch._C._cuda_getCurrentRawStream(first.get_device()):
-        for node, _ in first.grad_fn.next_functions:
-            if node is not None and hasattr(node, "variable"):
-                node.metadata[_EAGER] = True
-    return out
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 # ---- functions ------------------------------------------------------------------------------------------------------
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -498,12 +167,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     or None.  The result has x's type and shape."""
     if torch.compiler.is_compiling():
         return torch.ops.bilinear_hip.layer_norm(x, weight, bias, eps)[0]
-    _check_rows(x, "x")
-    _check_params(x, weight, bias)
-    _check_eps(eps)
-    if _wants_grad(x, weight, bias):
-        return _apply(_LayerNormFunction, (x, weight, bias), x, weight, bias, eps)
-    return _layer_norm(x, weight, bias, eps, save=False)[0]
+    return (_rows or _native()).layer_norm(x, weight, bias, eps)
 
 
 def dropout(x, p, seed, step=0, layer=0, row_offset=0, device_step=None):
@@ -514,11 +178,7 @@ def dropout(x, p, seed, step=0, layer=0, row_offset=0, device_step=None):
     that is added to ``step`` when the kernel runs: a captured graph that advances it draws another mask each replay."""
     if torch.compiler.is_compiling():
         return torch.ops.bilinear_hip.row_dropout(x, p, seed, step, layer, row_offset, device_step)[0]
-    _check_rows(x, "x")
-    _check_draws(p, seed, step, layer, row_offset, device_step, x)
-    if _wants_grad(x):
-        return _apply(_DropoutFunction, (x,), x, p, seed, step, layer, row_offset, device_step)
-    return _row_dropout(x, p, seed, step, layer, row_offset, device_step)[0]
+    return (_rows or _native()).dropout(x, p, seed, step, layer, row_offset, device_step)
 
 
 def residual_norm(x, residual, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, step=0, layer=0, row_offset=0,
@@ -529,15 +189,7 @@ def residual_norm(x, residual, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, 
     if torch.compiler.is_compiling():
         return torch.ops.bilinear_hip.residual_norm(x, residual, weight, bias, eps, p, seed, step, layer, row_offset,
                                                     device_step)[:2]
-    _check_rows(x, "x")
-    _check_like(residual, x, "residual", (x.dtype, torch.float32))
-    _check_params(x, weight, bias)
-    _check_eps(eps)
-    _check_draws(p, seed, step, layer, row_offset, device_step, x)
-    if _wants_grad(x, residual, weight, bias):
-        return _apply(_ResidualNormFunction, (x, residual, weight, bias), x, residual, weight, bias, eps, p, seed, step,
-                      layer, row_offset, device_step)
-    return _residual_norm(x, residual, weight, bias, eps, p, seed, step, layer, row_offset, device_step, save=False)[:2]
+    return (_rows or _native()).residual_norm(x, residual, weight, bias, eps, p, seed, step, layer, row_offset, device_step)
 
 
 # ---- modules --------------------------------------------------------------------------------------------------------
@@ -557,10 +209,11 @@ class LayerNorm(nn.LayerNorm):
 
 
 class _Draws:
-    """The seed, the step count and the stream id of a module that drops.  As for a stand-alone stage the seed is torch's
-    at the first call, the id is unique in the process (a copy gets its own) and the step counts calls; none is part of the
-    state_dict.  In a captured graph a step counted on the host would be frozen: give the module an int64 device tensor
-    (``set_device_step``) that the graph advances between replays."""
+    """The draws of a module that drops: torch's seed at the first call, a stream id that is unique in the process (a copy
+    gets its own, as every stand-alone stage does) and, as the step, a number from torch's CPU generator — so
+    ``torch.manual_seed`` repeats the masks, a saved generator state continues them and a checkpointed block (which
+    restores that state) is recomputed with the mask it had.  In a captured graph such a number would be frozen: give the
+    module an int64 device tensor (``set_device_step``) that the graph advances between replays."""
 
     _device_step = None
 
@@ -568,13 +221,13 @@ class _Draws:
         from .model.bilinear import _HeavyLinear
         self._layer = _HeavyLinear._next_stage_id[0]
         _HeavyLinear._next_stage_id[0] += 1
-        self._seed, self._step, self._captured = None, 0, 0
+        self._seed, self._captured = None, 0
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        step, seed = self._step, self._seed
+        seed = self._seed
         self._init_draws()
-        self._step, self._seed, self._device_step = step, seed, None
+        self._seed, self._device_step = seed, None
 
     def set_device_step(self, tensor):
         if tensor is not None and (tensor.dtype != torch.int64 or tensor.numel() != 1):
@@ -584,16 +237,15 @@ class _Draws:
     @torch.compiler.disable
     def _next_draws(self):
         if self._seed is None:
-            self._seed = int(torch.initial_seed()) & (_LIMIT63 - 1)
-        if torch.cuda.is_available() and _capturing():
+            self._seed = int(torch.initial_seed()) & ((1 << 63) - 1)
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             if self._device_step is None:
                 raise RuntimeError("bilinear_amd: dropout in a stream capture needs a step on the device "
                                    "(set_device_step): every replay would draw the same mask")
             # calls of one captured step differ in the upper half of the step, replays in the device's count
             self._captured += 1
             return {"seed": self._seed, "step": self._captured << 32, "layer": self._layer, "device_step": self._device_step}
-        self._step += 1
-        return {"seed": self._seed, "step": self._step - 1, "layer": self._layer}
+        return {"seed": self._seed, "step": int(torch.empty((), dtype=torch.int64).random_()), "layer": self._layer}
 
 
 class Dropout(_Draws, nn.Dropout):

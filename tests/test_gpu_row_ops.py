@@ -155,6 +155,75 @@ def test_only_the_gradients_that_are_wanted(B):
     assert torch.equal(torch.autograd.grad(B.layer_norm(x.detach(), w.detach(), b), b, dy)[0], full[2])
 
 
+def test_parameters_that_are_not_dense(B):
+    w, b = params(2 * 300, F32, 5)
+    x, dy = data(7, 300, F32, 1).requires_grad_(), data(7, 300, F32, 2)
+    for p, q in ((w[::2], b[1::2]), (w.view(300, 2)[:, 1], b[:1].expand(300))):
+        got = torch.autograd.grad(B.layer_norm(x, p, q), (x, w, b), dy)
+        want = torch.autograd.grad(B.layer_norm(x, p.contiguous(), q.contiguous()), (x, w, b), dy)
+        for u, v in zip(got, want):
+            assert torch.equal(u, v)
+
+
+def test_graphs_kept_freed_and_written_to(B):
+    x, r, dy = data(20, 64, F32, 1).requires_grad_(), data(20, 64, F32, 2).requires_grad_(), data(20, 64, F32, 3)
+    y, h = B.residual_norm(x, r, p=0.3, seed=1)
+    once = torch.autograd.grad((y, h), (x, r), (dy, dy), retain_graph=True)
+    for p, q in zip(once, torch.autograd.grad((y, h), (x, r), (dy, dy))):
+        assert torch.equal(p, q)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad((y, h), (x, r), (dy, dy))
+    y, h = B.residual_norm(x, r, p=0.3, seed=1)
+    h.add_(1)                                 # what the backward reads: refused by its version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, x, dy)
+    z = B.layer_norm(x)
+    z.mul_(2)                                 # nothing reads y: this stays a plain factor
+    assert torch.equal(torch.autograd.grad(z, x, dy)[0], torch.autograd.grad(B.layer_norm(x), x, 2 * dy)[0])
+
+
+def test_a_checkpointed_block_is_recomputed_with_its_mask(B):
+    from torch.utils.checkpoint import checkpoint
+    x, dy = data(40, 64, F32, 1).requires_grad_(), data(40, 64, F32, 2)
+    norm, drop = B.ResidualNorm(64, p=0.4).cuda(), B.Dropout(0.4)
+    block = lambda t: drop(norm(t, t)[0])     # noqa: E731
+    torch.manual_seed(8)
+    want = torch.autograd.grad(block(x), (x, norm.weight), dy)
+    for reentrant in (False, True):
+        torch.manual_seed(8)
+        out = checkpoint(block, x, use_reentrant=reentrant)
+        x.grad = norm.weight.grad = None
+        out.backward(dy)
+        assert torch.equal(x.grad, want[0]) and torch.equal(norm.weight.grad, want[1])
+
+
+def test_a_second_thread_and_single_threaded_backward(B):
+    import threading
+    x, dy = data(500, 300, BF16, 1), data(500, 300, BF16, 2)
+    w, b = params(300, F32, 5)
+
+    def work():
+        t = x.detach().requires_grad_()
+        return torch.autograd.grad(B.layer_norm(t, w, b), (t, w, b), dy)
+
+    want, got = work(), [None] * 4
+    torch.cuda.synchronize()
+
+    def run(i):
+        got[i] = work()
+        torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    with torch.autograd.set_multithreading_enabled(False):
+        got.append(work())
+    for g in got:
+        for p, q in zip(g, want):
+            assert torch.equal(p, q)
+
+
 def test_double_backward_is_refused(B):
     x = data(3, 16, F32, 1).requires_grad_()
     g, = torch.autograd.grad(B.layer_norm(x).square().sum(), x, create_graph=True)
@@ -486,9 +555,10 @@ def test_a_residual_network_of_the_operators_trains(B):
 
     net = Net().cuda()
     x, t = data(rows, 32, F32, 1), data(rows, 48, F32, 2)
-    seed = torch.initial_seed() & ((1 << 63) - 1)
-    masks = [R.factor(rows, width, p, seed=seed, layer=m._layer) for m in [net.drop, *net.norms]]
+    state = torch.get_rng_state()
     torch.nn.functional.mse_loss(net(x), t).backward()
+    torch.set_rng_state(state)                # the numbers the modules drew, in the order of their calls
+    masks = [R.factor(rows, width, p, **m._next_draws()) for m in [net.drop, *net.norms]]
 
     P = {k: v.detach().double().cpu().requires_grad_() for k, v in net.named_parameters()}
     h = (d(x) @ P["encode.weight"].t() + P["encode.bias"]) * masks[0]
