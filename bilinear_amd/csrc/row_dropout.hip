@@ -22,26 +22,38 @@ int row_make_drop(const blh_row_drop* d, int64_t rows, RowDrop* out) {
   return BLH_OK;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void row_dropout_kernel(const T* x, int64_t ldx, T* y, RowDrop drop, int64_t rows,
-                                                          int64_t width, int64_t units) {
+// I: the type that counts units (32 bits wherever they fit: the division by `units` is what the index costs)
+template <typename T, typename I, bool SHORT>
+__global__ __launch_bounds__(256) void row_dropout_kernel(const T* x, int64_t ldx, T* y, RowDrop drop, I total, I units,
+                                                          int width) {
   const RowKey key = row_key(drop);
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * units; i += gridDim.x * 256ll) {
-    const int64_t row = i / units, unit = i - row * units, col = unit * ROW_UNIT;
+  for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {
+    const I row = i / units;
+    const int unit = (int)(i - row * units), c = unit * ROW_UNIT;
     float f[ROW_UNIT];
-    load_unit(x + row * ldx + col, width - col, f);
-    drop_unit(key, drop, drop.row_offset + row, unit, f);
-    store_unit(y + row * width + col, width - col, f);
+    load_unit<SHORT>(x + (int64_t)row * ldx, c, width, f);
+    drop_unit(key, drop, drop.row_offset + (int64_t)row, unit, f);
+    store_unit(y + (int64_t)row * width, c, width, f);
   }
 }
 
 template <typename T>
 static int launch_row_dropout(hipStream_t s, const void* x, int64_t ldx, void* y, const RowDrop& drop, int64_t rows,
                               int64_t width) {
-  const int64_t units = ceil_div(width, ROW_UNIT);
-  const int64_t blocks = std::min<int64_t>(ceil_div(rows * units, 256), 4096);
-  hipLaunchKernelGGL((row_dropout_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T*>(x), ldx,
-                     static_cast<T*>(y), drop, rows, width, units);
+  const int64_t units = ceil_div(width, ROW_UNIT), total = rows * units;
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(total, 256), 4096);
+  const T* in = static_cast<const T*>(x);
+  T* out = static_cast<T*>(y);
+  // (32 bits: the loop's index passes `total` by at most one grid)
+  if (width < ROW_UNIT)
+    hipLaunchKernelGGL((row_dropout_kernel<T, uint64_t, true>), dim3(blocks), dim3(256), 0, s, in, ldx, out, drop,
+                       (uint64_t)total, (uint64_t)units, (int)width);
+  else if (total < (int64_t)1 << 31)
+    hipLaunchKernelGGL((row_dropout_kernel<T, uint32_t, false>), dim3(blocks), dim3(256), 0, s, in, ldx, out, drop,
+                       (uint32_t)total, (uint32_t)units, (int)width);
+  else
+    hipLaunchKernelGGL((row_dropout_kernel<T, uint64_t, false>), dim3(blocks), dim3(256), 0, s, in, ldx, out, drop,
+                       (uint64_t)total, (uint64_t)units, (int)width);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
 }

@@ -48,33 +48,33 @@ template <typename T, typename R, bool RESID>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormFwd p) {
   __shared__ float sh[4];
   const RowKey key = RESID && p.drop.threshold ? row_key(p.drop) : RowKey{};
-  const int64_t W = p.width, units = (W + ROW_UNIT - 1) / ROW_UNIT;
+  const int W = (int)p.width, units = (W + ROW_UNIT - 1) / ROW_UNIT;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    T* y = static_cast<T*>(p.y) + row * W;
-    R* h = RESID ? static_cast<R*>(p.h) + row * W : nullptr;
+    T* y = static_cast<T*>(p.y) + row * p.width;
+    R* h = RESID ? static_cast<R*>(p.h) + row * p.width : nullptr;
     float sum = 0.f;
-    for (int64_t u = threadIdx.x; u < units; u += 256) {
+    for (int u = threadIdx.x; u < units; u += 256) {
       float f[ROW_UNIT];
-      const int64_t c = u * ROW_UNIT;
-      load_unit(x + c, W - c, f);
+      const int c = u * ROW_UNIT;
+      load_unit<false>(x, c, W, f);
       if (RESID) {
         float r[ROW_UNIT];
-        load_unit(static_cast<const R*>(p.res) + row * p.ldr + c, W - c, r);
+        load_unit<false>(static_cast<const R*>(p.res) + row * p.ldr, c, W, r);
         drop_add_unit(key, p.drop, p.drop.row_offset + row, u, r, f);
 #pragma unroll
         for (int e = 0; e < ROW_UNIT; ++e) f[e] = (float)(R)f[e];      // (what the stream holds is what is normalised)
-        store_unit(h + c, W - c, f);
+        store_unit(h, c, W, f);
       }
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e) sum += f[e];
     }
     const float mean = block_sum(sum, sh) / (float)W;
     float sq = 0.f;
-    for (int64_t u = threadIdx.x; u < units; u += 256) {
+    for (int u = threadIdx.x; u < units; u += 256) {
       float f[ROW_UNIT];
-      const int64_t c = u * ROW_UNIT;
-      if (RESID) load_unit(h + c, W - c, f); else load_unit(x + c, W - c, f);
+      const int c = u * ROW_UNIT;
+      if (RESID) load_unit<false>(h, c, W, f); else load_unit<false>(x, c, W, f);
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e) {
         const float d = c + e < W ? f[e] - mean : 0.f;
@@ -83,15 +83,15 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormFwd p) {
     }
     const float rstd = 1.f / sqrtf(block_sum(sq, sh) / (float)W + p.eps);
     if (threadIdx.x == 0 && p.mean) { p.mean[row] = mean; p.rstd[row] = rstd; }
-    for (int64_t u = threadIdx.x; u < units; u += 256) {
+    for (int u = threadIdx.x; u < units; u += 256) {
       float f[ROW_UNIT], g[ROW_UNIT], b[ROW_UNIT];
-      const int64_t c = u * ROW_UNIT;
-      if (RESID) load_unit(h + c, W - c, f); else load_unit(x + c, W - c, f);
-      load_param_unit<T>(p.gamma, p.same, c, W - c, 1.f, g);
-      load_param_unit<T>(p.beta, p.same, c, W - c, 0.f, b);
+      const int c = u * ROW_UNIT;
+      if (RESID) load_unit<false>(h, c, W, f); else load_unit<false>(x, c, W, f);
+      load_param_unit<false, T>(p.gamma, p.same, c, W, 1.f, g);
+      load_param_unit<false, T>(p.beta, p.same, c, W, 0.f, b);
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e) f[e] = fmaf((f[e] - mean) * rstd, g[e], b[e]);
-      store_unit(y + c, W - c, f);
+      store_unit(y, c, W, f);
     }
   }
 }
@@ -101,18 +101,18 @@ template <typename T, typename R, bool RESID>
 __global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormBwd p) {
   __shared__ float sh[4];
   const RowKey key = RESID && p.drop.threshold ? row_key(p.drop) : RowKey{};
-  const int64_t W = p.width, units = (W + ROW_UNIT - 1) / ROW_UNIT;
+  const int W = (int)p.width, units = (W + ROW_UNIT - 1) / ROW_UNIT;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
     const R* h = static_cast<const R*>(p.h) + row * p.ldh;
     const float mean = p.mean[row], rstd = p.rstd[row];
     float s1 = 0.f, s2 = 0.f;
-    for (int64_t u = threadIdx.x; u < units; u += 256) {
+    for (int u = threadIdx.x; u < units; u += 256) {
       float d[ROW_UNIT], f[ROW_UNIT], g[ROW_UNIT];
-      const int64_t c = u * ROW_UNIT;
-      load_unit(dy + c, W - c, d);
-      load_unit(h + c, W - c, f);
-      load_param_unit<T>(p.gamma, p.same, c, W - c, 1.f, g);
+      const int c = u * ROW_UNIT;
+      load_unit<false>(dy, c, W, d);
+      load_unit<false>(h, c, W, f);
+      load_param_unit<false, T>(p.gamma, p.same, c, W, 1.f, g);
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e) {
         const float t = d[e] * g[e];          // (zero behind the row's end: dy is)
@@ -122,25 +122,25 @@ __global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormBwd p) {
     }
     const float c1 = block_sum(s1, sh) / (float)W;
     const float c2 = block_sum(s2, sh) / (float)W;
-    for (int64_t u = threadIdx.x; u < units; u += 256) {
+    for (int u = threadIdx.x; u < units; u += 256) {
       float d[ROW_UNIT], f[ROW_UNIT], g[ROW_UNIT];
-      const int64_t c = u * ROW_UNIT;
-      load_unit(dy + c, W - c, d);
-      load_unit(h + c, W - c, f);
-      load_param_unit<T>(p.gamma, p.same, c, W - c, 1.f, g);
+      const int c = u * ROW_UNIT;
+      load_unit<false>(dy, c, W, d);
+      load_unit<false>(h, c, W, f);
+      load_param_unit<false, T>(p.gamma, p.same, c, W, 1.f, g);
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e)
         f[e] = rstd * (d[e] * g[e] - c1 - (f[e] - mean) * rstd * c2);
       if (RESID) {
         if (p.dh) {
-          load_unit(static_cast<const R*>(p.dh) + row * p.lddh + c, W - c, g);
+          load_unit<false>(static_cast<const R*>(p.dh) + row * p.lddh, c, W, g);
 #pragma unroll
           for (int e = 0; e < ROW_UNIT; ++e) f[e] += g[e];
         }
-        if (p.dres) store_unit(static_cast<R*>(p.dres) + row * W + c, W - c, f);
+        if (p.dres) store_unit(static_cast<R*>(p.dres) + row * p.width, c, W, f);
         if (p.drop.threshold) drop_unit(key, p.drop, p.drop.row_offset + row, u, f);
       }
-      if (p.dx) store_unit(static_cast<T*>(p.dx) + row * W + c, W - c, f);
+      if (p.dx) store_unit(static_cast<T*>(p.dx) + row * p.width, c, W, f);
     }
   }
 }
@@ -150,13 +150,13 @@ template <typename T, typename R>
 __global__ __launch_bounds__(256) void norm_bwd_cols_kernel(NormBwd p) {
   __shared__ float sh[4][2][64 * ROW_UNIT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t W = p.width, c0 = (int64_t)blockIdx.x * 64 * ROW_UNIT, c = c0 + lane * ROW_UNIT;
+  const int W = (int)p.width, c0 = blockIdx.x * 64 * ROW_UNIT, c = c0 + lane * ROW_UNIT;
   const int64_t r0 = blockIdx.y * p.chunk, r1 = min(p.rows, r0 + p.chunk);
   float ag[ROW_UNIT] = {}, ab[ROW_UNIT] = {};
   for (int64_t row = r0 + wave; row < r1; row += 4) {
     float d[ROW_UNIT], f[ROW_UNIT];
-    load_unit(static_cast<const T*>(p.dy) + row * p.lddy + c, W - c, d);
-    load_unit(static_cast<const R*>(p.h) + row * p.ldh + c, W - c, f);
+    load_unit<false>(static_cast<const T*>(p.dy) + row * p.lddy, c, W, d);
+    load_unit<false>(static_cast<const R*>(p.h) + row * p.ldh, c, W, f);
     const float mean = p.mean[row], rstd = p.rstd[row];
 #pragma unroll
     for (int e = 0; e < ROW_UNIT; ++e) {
@@ -226,7 +226,7 @@ template <int LANES> struct RowGroup {
       __syncthreads();
       a = b = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) { const float2 v = sh[turn][w]; a += v.x; b += v.y; }
+      for (int w = 0; w < WAVES; ++w) { const float2 v = sh[turn][(wave & ~(WAVES - 1)) + w]; a += v.x; b += v.y; }
       turn ^= 1;
     }
   }
@@ -239,51 +239,62 @@ template <int LANES> struct RowGroup {
       __syncthreads();
       a = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) a += sh[turn][w].x;
+      for (int w = 0; w < WAVES; ++w) a += sh[turn][(wave & ~(WAVES - 1)) + w].x;
       turn ^= 1;
     }
     return a;
   }
 };
 
-template <int LANES> constexpr int fwd_block() { return LANES > 256 ? LANES : 256; }
-
-template <typename T, typename R, bool RESID, int LANES, int NV>
-__global__ __launch_bounds__(fwd_block<LANES>()) void norm_fwd_rows_kernel(NormFwd p) {
-  constexpr int BLOCK = fwd_block<LANES>(), GROUPS = BLOCK / LANES;
+template <typename T, typename R, bool RESID, int LANES, int NV, int BLOCK, bool SHORT>
+__global__ __launch_bounds__(BLOCK) void norm_fwd_rows_kernel(NormFwd p) {
+  constexpr int GROUPS = BLOCK / LANES;
   __shared__ float2 sh[2][16];
   RowGroup<LANES> group;
   const RowKey key = RESID && p.drop.threshold ? row_key(p.drop) : RowKey{};
   const int W = (int)p.width, lane = threadIdx.x % LANES;
   int g = threadIdx.x / LANES;
   if constexpr (LANES == 64) g = __builtin_amdgcn_readfirstlane(g);
-  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
-    const int64_t row = base + g;
-    const int width = row < p.rows ? W : 0;        // (a group behind the last row: nothing is read or written)
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    float f[NV][ROW_UNIT];
-    RawUnit<T> xr[NV];
-    RawUnit<R> rr[RESID ? NV : 1];
+  // the parameters first: in the epilogue each would be a round trip of its own, behind the sums
+  float gm[NV][ROW_UNIT], bt[NV][ROW_UNIT];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + lane) * ROW_UNIT;
+    load_param_unit<SHORT, T>(p.gamma, p.same, c, W, 1.f, gm[i]);
+    load_param_unit<SHORT, T>(p.beta, p.same, c, W, 0.f, bt[i]);
+  }
+  struct In { RawUnit<T> x[NV]; RawUnit<R> r[RESID ? NV : 1]; };
+  auto load = [&](int64_t row, In& q) {
+    row = min(row, p.rows - 1);                    // (a group behind the last row reads that one and writes nothing)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * ROW_UNIT;
-      xr[i] = load_raw(x + c, width - c);
-      if constexpr (RESID) rr[i] = load_raw(static_cast<const R*>(p.res) + row * p.ldr + c, width - c);
+      q.x[i] = load_raw<SHORT>(static_cast<const T*>(p.x) + row * p.ldx, c, W);
+      if constexpr (RESID) q.r[i] = load_raw<SHORT>(static_cast<const R*>(p.res) + row * p.ldr, c, W);
     }
+  };
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
+    const int64_t row = base + g;
+    const int width = row < p.rows ? W : 0;
+    In in;
+    load(row, in);
+    float f[NV][ROW_UNIT];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = i * LANES + lane, c = u * ROW_UNIT;
+      settle(in.x[i], c, width);
 #pragma unroll
-      for (int e = 0; e < ROW_UNIT; ++e) f[i][e] = xr[i].get(e);
+      for (int e = 0; e < ROW_UNIT; ++e) f[i][e] = in.x[i].get(e);
       if constexpr (RESID) {
         float r[ROW_UNIT];
+        settle(in.r[i], c, width);
 #pragma unroll
-        for (int e = 0; e < ROW_UNIT; ++e) r[e] = rr[i].get(e);
+        for (int e = 0; e < ROW_UNIT; ++e) r[e] = in.r[i].get(e);
         drop_add_unit(key, p.drop, p.drop.row_offset + row, u, r, f[i]);
 #pragma unroll
         for (int e = 0; e < ROW_UNIT; ++e) f[i][e] = (float)(R)f[i][e];      // (what the stream holds is what is normalised)
-        store_unit(static_cast<R*>(p.h) + row * p.width + c, width - c, f[i]);
+        store_unit(static_cast<R*>(p.h) + row * p.width, c, width, f[i]);
       }
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e) sum += f[i][e];
@@ -304,164 +315,176 @@ __global__ __launch_bounds__(fwd_block<LANES>()) void norm_fwd_rows_kernel(NormF
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * ROW_UNIT;
-      float gm[ROW_UNIT], bt[ROW_UNIT];
-      load_param_unit<T>(p.gamma, p.same, c, width - c, 1.f, gm);
-      load_param_unit<T>(p.beta, p.same, c, width - c, 0.f, bt);
 #pragma unroll
-      for (int e = 0; e < ROW_UNIT; ++e) f[i][e] = fmaf(f[i][e] * rstd, gm[e], bt[e]);
-      store_unit(static_cast<T*>(p.y) + row * p.width + c, width - c, f[i]);
+      for (int e = 0; e < ROW_UNIT; ++e) f[i][e] = fmaf(f[i][e] * rstd, gm[i][e], bt[i][e]);
+      store_unit(static_cast<T*>(p.y) + row * p.width, c, width, f[i]);
     }
   }
 }
 
-// One block's rows: dh' (and dx), and the block's partial column sums.
-template <typename T, typename R, bool RESID, int LANES, int NV, int BLOCK>
+// partial rows a block of the backward holds in LDS: one for each wave (groups inside a wave join by shuffles) or for each
+// group of waves, but the first, which stays in registers
+template <int LANES, int BLOCK> constexpr int bwd_shares() { return LANES < 64 ? BLOCK / 64 : BLOCK / LANES; }
+
+// One block's rows, a unit a lane: dh' (and dx), and the block's partial column sums in its row of p.part.
+template <typename T, typename R, bool RESID, int LANES, int BLOCK, bool SHORT>
 __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
-  constexpr int GROUPS = BLOCK / LANES;
+  constexpr int GROUPS = BLOCK / LANES, SHARES = bwd_shares<LANES, BLOCK>();
   __shared__ float2 sh[2][16];
-  extern __shared__ float cols[];          // [2][stride]
+  extern __shared__ f32x4 cols4[];         // [SHARES - 1][2][stride]
   RowGroup<LANES> group;
   const RowKey key = RESID && p.drop.threshold ? row_key(p.drop) : RowKey{};
-  const int W = (int)p.width, lane = threadIdx.x % LANES;
+  const int W = (int)p.width, u = threadIdx.x % LANES, c = u * ROW_UNIT;
   int g = threadIdx.x / LANES;
   if constexpr (LANES == 64) g = __builtin_amdgcn_readfirstlane(g);
-  float gm[NV][ROW_UNIT], ag[NV][ROW_UNIT], ab[NV][ROW_UNIT];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * LANES + lane) * ROW_UNIT;
-    load_param_unit<T>(p.gamma, p.same, c, W - c, 1.f, gm[i]);
-#pragma unroll
-    for (int e = 0; e < ROW_UNIT; ++e) ag[i][e] = ab[i][e] = 0.f;
-  }
-  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
+  float gm[ROW_UNIT], ag[ROW_UNIT] = {}, ab[ROW_UNIT] = {};
+  load_param_unit<SHORT, T>(p.gamma, p.same, c, W, 1.f, gm);
+  struct In { RawUnit<T> d; RawUnit<R> f, dh; float mean, rstd; };
+  auto load = [&](int64_t row, In& q) {
+    row = min(row, p.rows - 1);                    // (a group behind the last row reads that one and writes nothing)
+    q.d = load_raw<SHORT>(static_cast<const T*>(p.dy) + row * p.lddy, c, W);
+    q.f = load_raw<SHORT>(static_cast<const R*>(p.h) + row * p.ldh, c, W);
+    if (RESID && p.dh) q.dh = load_raw<SHORT>(static_cast<const R*>(p.dh) + row * p.lddh, c, W);
+    q.mean = p.mean[row];
+    q.rstd = p.rstd[row];
+  };
+  // the next row's loads go out in front of this row's sums where that costs at most 12 registers (16384 x 1024 bf16: 21.9
+  // against 22.9 us; with an fp32 stream the registers cost more waves than the loads bring: 8192 x 1024 36.3 against 35.2)
+  constexpr bool AHEAD = sizeof(T) + (RESID ? 2 : 1) * sizeof(R) <= 6;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  In next;
+  if constexpr (AHEAD) load((int64_t)blockIdx.x * GROUPS + g, next);
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += step) {
     const int64_t row = base + g;
-    const bool live = row < p.rows;
-    const int width = live ? W : 0;
-    const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
-    const R* h = static_cast<const R*>(p.h) + row * p.ldh;
-    RawUnit<T> d[NV];
-    RawUnit<R> f[NV], dh[RESID ? NV : 1];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * ROW_UNIT;
-      d[i] = load_raw(dy + c, width - c);
-      f[i] = load_raw(h + c, width - c);
+    const int width = row < p.rows ? W : 0;
+    In in;
+    if constexpr (AHEAD) {
+      in = next;
+      if (base + step < p.rows) load(row + step, next);
+    } else {
+      load(row, in);
     }
-    if constexpr (RESID) {
-      if (p.dh) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (i * LANES + lane) * ROW_UNIT;
-          dh[i] = load_raw(static_cast<const R*>(p.dh) + row * p.lddh + c, width - c);
-        }
-      }
-    }
-    const float mean = live ? p.mean[row] : 0.f, rstd = live ? p.rstd[row] : 0.f;
+    settle(in.d, c, width);                        // (dy is 0 behind the row's end)
+    settle(in.f, c, width);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int e = 0; e < ROW_UNIT; ++e) {
-        const float v = d[i].get(e), hat = (f[i].get(e) - mean) * rstd, t = v * gm[i][e];     // (v = 0 behind the row's end)
-        s1 += t;
-        s2 = fmaf(t, hat, s2);
-        ag[i][e] = fmaf(v, hat, ag[i][e]);
-        ab[i][e] += v;
-      }
+    for (int e = 0; e < ROW_UNIT; ++e) {
+      const float v = in.d.get(e), hat = (in.f.get(e) - in.mean) * in.rstd, t = v * gm[e];
+      s1 += t;
+      s2 = fmaf(t, hat, s2);
+      ag[e] = fmaf(v, hat, ag[e]);
+      ab[e] += v;
     }
     group.sum2(s1, s2, sh);
     const float c1 = s1 / (float)W, c2 = s2 / (float)W;
+    float o[ROW_UNIT];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int u = i * LANES + lane, c = u * ROW_UNIT;
-      float o[ROW_UNIT];
-#pragma unroll
-      for (int e = 0; e < ROW_UNIT; ++e) {
-        const float hat = (f[i].get(e) - mean) * rstd;
-        o[e] = rstd * (fmaf(d[i].get(e), gm[i][e], -c1) - hat * c2);
-      }
-      if constexpr (RESID) {
-        if (p.dh) {
-#pragma unroll
-          for (int e = 0; e < ROW_UNIT; ++e) o[e] += dh[i].get(e);
-        }
-        if (p.dres) store_unit(static_cast<R*>(p.dres) + row * p.width + c, width - c, o);
-        if (p.dx && p.drop.threshold) drop_unit(key, p.drop, p.drop.row_offset + row, u, o);
-      }
-      if (p.dx) store_unit(static_cast<T*>(p.dx) + row * p.width + c, width - c, o);
+    for (int e = 0; e < ROW_UNIT; ++e) {
+      const float hat = (in.f.get(e) - in.mean) * in.rstd;
+      o[e] = in.rstd * (fmaf(in.d.get(e), gm[e], -c1) - hat * c2);
     }
+    if constexpr (RESID) {
+      if (p.dh) {
+        settle(in.dh, c, width);
+#pragma unroll
+        for (int e = 0; e < ROW_UNIT; ++e) o[e] += in.dh.get(e);
+      }
+      if (p.dres) store_unit(static_cast<R*>(p.dres) + row * p.width, c, width, o);
+      if (p.dx && p.drop.threshold) drop_unit(key, p.drop, p.drop.row_offset + row, u, o);
+    }
+    if (p.dx) store_unit(static_cast<T*>(p.dx) + row * p.width, c, width, o);
   }
   if (!p.part) return;
-  // the block's groups add their columns up one after the other
-#pragma unroll 1
-  for (int k = 0; k < GROUPS; ++k) {
-    if (k == threadIdx.x / LANES) {
+  if constexpr (LANES < 64) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (i * LANES + lane) * ROW_UNIT;
-        if (c < W) {
+    for (int e = 0; e < ROW_UNIT; ++e)
 #pragma unroll
-          for (int e = 0; e < ROW_UNIT; ++e) {
-            cols[c + e] = k ? cols[c + e] + ag[i][e] : ag[i][e];
-            cols[p.stride + c + e] = k ? cols[p.stride + c + e] + ab[i][e] : ab[i][e];
-          }
-        }
+      for (int o = LANES; o < 64; o <<= 1) {
+        ag[e] += __shfl_xor(ag[e], o);
+        ab[e] += __shfl_xor(ab[e], o);
       }
+  }
+  const int share = LANES < 64 ? threadIdx.x >> 6 : threadIdx.x / LANES;
+  const bool mine = (LANES >= 64 || (threadIdx.x & 63) < LANES) && c < W;
+  f32x4 a[4] = {{ag[0], ag[1], ag[2], ag[3]}, {ag[4], ag[5], ag[6], ag[7]},
+                {ab[0], ab[1], ab[2], ab[3]}, {ab[4], ab[5], ab[6], ab[7]}};
+  const int64_t at[4] = {c / 4, c / 4 + 1, (p.stride + c) / 4, (p.stride + c) / 4 + 1};
+  if constexpr (SHARES > 1) {
+    if (mine && share > 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cols4[(share - 1) * (p.stride / 2) + at[i]] = a[i];
     }
     __syncthreads();
   }
-  float* out = p.part + (int64_t)blockIdx.x * 2 * p.stride;
-  for (int j = threadIdx.x * 4; j < 2 * p.stride; j += BLOCK * 4)
-    *reinterpret_cast<f32x4*>(out + j) = *reinterpret_cast<const f32x4*>(cols + j);
+  if (mine && share == 0) {
+    f32x4* out = reinterpret_cast<f32x4*>(p.part + (int64_t)blockIdx.x * 2 * p.stride);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int k = 1; k < SHARES; ++k) a[i] += cols4[(k - 1) * (p.stride / 2) + at[i]];
+      out[at[i]] = a[i];
+    }
+  }
 }
 
 // rows of one partial sum of the wide form: whole groups of 16 rows, at most 256 chunks
 static int64_t norm_chunk(int64_t rows) { return round_up(std::max<int64_t>(1, ceil_div(rows, 256)), 16); }
 static int64_t norm_stride(int64_t width) { return round_up(width, ROW_UNIT); }
 static constexpr int64_t ROW_RESIDENT = 8192;      // widest row that stays in registers
-#ifndef ROW_BWD_BLOCKS
-#define ROW_BWD_BLOCKS 512
-#endif
-#ifndef ROW_FWD_BLOCKS
-#define ROW_FWD_BLOCKS 2048
-#endif
-static constexpr int BWD_BLOCKS = ROW_BWD_BLOCKS;      // partial rows the backward leaves at most
+// Blocks of the resident backward: 16 waves a CU, in two blocks of 512 threads, or in one of 1024 where a row is over 1024
+// columns and its partial sums are the larger cost (16384 x 2048 bf16 residual norm 65.3 against 68.4 us, 8192 x 4096 67.2
+// against 72.8; 1024 blocks of 256 threads 73).
+static constexpr int64_t ROW_TWO_BLOCKS = 1024;
+static int norm_blocks(int64_t width) { return width <= ROW_TWO_BLOCKS ? 512 : 256; }
 static int norm_partials(int64_t rows, int64_t width) {
-  return width <= ROW_RESIDENT ? (int)std::min<int64_t>(rows, BWD_BLOCKS) : (int)ceil_div(rows, norm_chunk(rows));
+  return (int)(width <= ROW_RESIDENT ? std::min<int64_t>(rows, norm_blocks(width)) : ceil_div(rows, norm_chunk(rows)));
 }
 
-template <typename T, typename R, bool RESID, int LANES, int NV>
+template <typename T, typename R, bool RESID, int LANES, int NV, bool SHORT = false>
 static int launch_fwd_rows(hipStream_t s, const NormFwd& p) {
-  constexpr int BLOCK = fwd_block<LANES>();
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), ROW_FWD_BLOCKS);
-  hipLaunchKernelGGL((norm_fwd_rows_kernel<T, R, RESID, LANES, NV>), dim3(blocks), dim3(BLOCK), 0, s, p);
+  constexpr int BLOCK = LANES > 256 ? LANES : 256;
+  // at most 8 blocks of 256 threads a CU, which walk the rows with the parameters in registers: 16384 x 2048 bf16 layer
+  // norm 22.4 us, one group of rows a block (parameters read for each) 27.6
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), 2048 * 256 / BLOCK);
+  hipLaunchKernelGGL((norm_fwd_rows_kernel<T, R, RESID, LANES, NV, BLOCK, SHORT>), dim3(blocks), dim3(BLOCK), 0, s, p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
 }
 
+// Lanes a row.  16-bit rows of up to 2048 columns belong to one wave (two for the residual norm, which holds two streams) of
+// 2 or 4 units a lane: no barrier, and the parameters' registers are spent once per row in flight (16384 x 2048 bf16:
+// 22.4 us, spread over four waves 25.0).  fp32 rows are twice the bytes and go to twice the lanes (8192 x 1024: 12.6 against
+// 14.0 us).  Few rows — at most eight a CU — are spread too, one unit a lane: nothing else hides a row's latency (1 x 2048
+// residual norm 5.3 us, by one wave 8.3).
 template <typename T, typename R, bool RESID>
 static int launch_norm_fwd(hipStream_t s, const NormFwd& p) {
+  constexpr bool wide = sizeof(T) == 4;
+  const bool few = p.rows <= 2048;
+  if (p.width < ROW_UNIT) return launch_fwd_rows<T, R, RESID, 16, 1, true>(s, p);
   if (p.width <= 128) return launch_fwd_rows<T, R, RESID, 16, 1>(s, p);
   if (p.width <= 256) return launch_fwd_rows<T, R, RESID, 32, 1>(s, p);
   if (p.width <= 512) return launch_fwd_rows<T, R, RESID, 64, 1>(s, p);
-  if (p.width <= 1024) return launch_fwd_rows<T, R, RESID, 64, 2>(s, p);
-  if (p.width <= 2048) return launch_fwd_rows<T, R, RESID, 64, 4>(s, p);
-  if (p.width <= 4096) return launch_fwd_rows<T, R, RESID, 256, 2>(s, p);
-  if (p.width <= ROW_RESIDENT) return launch_fwd_rows<T, R, RESID, 256, 4>(s, p);
+  if (p.width <= 1024) {
+    if (wide || few) return launch_fwd_rows<T, R, RESID, 128, 1>(s, p);
+    if constexpr (!wide) return launch_fwd_rows<T, R, RESID, 64, 2>(s, p);
+  }
+  if (p.width <= 2048) {
+    if (wide || few) return launch_fwd_rows<T, R, RESID, 256, 1>(s, p);
+    if constexpr (!wide) return launch_fwd_rows<T, R, RESID, RESID ? 128 : 64, RESID ? 2 : 4>(s, p);
+  }
+  if (p.width <= 4096) return launch_fwd_rows<T, R, RESID, wide ? 512 : 256, wide ? 1 : 2>(s, p);
+  if (p.width <= ROW_RESIDENT) return launch_fwd_rows<T, R, RESID, wide ? 512 : 256, wide ? 2 : 4>(s, p);
   const unsigned blocks = (unsigned)std::min<int64_t>(p.rows, 1 << 16);
   hipLaunchKernelGGL((norm_fwd_kernel<T, R, RESID>), dim3(blocks), dim3(256), 0, s, p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
 }
 
-template <typename T, typename R, bool RESID, int LANES, int NV, int BLOCK>
+template <typename T, typename R, bool RESID, int LANES, int BLOCK, bool SHORT = false>
 static int launch_bwd_rows(hipStream_t s, NormBwd& p) {
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), BWD_BLOCKS);
-  p.chunks = (int)blocks;
-  const size_t lds = p.part ? 2 * p.stride * sizeof(float) : 0;
-  auto kern = norm_bwd_kernel<T, R, RESID, LANES, NV, BLOCK>;
-  if (lds > 65536 - 1024) BLH_HIP_TRY(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  hipLaunchKernelGGL(kern, dim3(blocks), dim3(BLOCK), lds, s, p);
+  p.chunks = (int)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), norm_blocks(p.width));
+  const size_t lds = p.part ? (bwd_shares<LANES, BLOCK>() - 1) * 2 * p.stride * sizeof(float) : 0;    // at most 48 KiB
+  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, BLOCK, SHORT>), dim3((unsigned)p.chunks), dim3(BLOCK), lds, s, p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
 }
@@ -472,13 +495,14 @@ static int launch_norm_bwd(hipStream_t s, NormBwd p) {
   p.stride = norm_stride(p.width);
   if (!grads) p.part = nullptr;
   if (p.rows > 0 && p.width <= ROW_RESIDENT) {
-    if (p.width <= 128) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 1, 256>(s, p)));
-    else if (p.width <= 256) BLH_TRY((launch_bwd_rows<T, R, RESID, 32, 1, 256>(s, p)));
-    else if (p.width <= 512) BLH_TRY((launch_bwd_rows<T, R, RESID, 64, 1, 512>(s, p)));
-    else if (p.width <= 1024) BLH_TRY((launch_bwd_rows<T, R, RESID, 64, 2, 512>(s, p)));
-    else if (p.width <= 2048) BLH_TRY((launch_bwd_rows<T, R, RESID, 64, 4, 512>(s, p)));
-    else if (p.width <= 4096) BLH_TRY((launch_bwd_rows<T, R, RESID, 256, 2, 256>(s, p)));
-    else BLH_TRY((launch_bwd_rows<T, R, RESID, 256, 4, 256>(s, p)));
+    if (p.width < ROW_UNIT) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 512, true>(s, p)));
+    else if (p.width <= 128) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 512>(s, p)));
+    else if (p.width <= 256) BLH_TRY((launch_bwd_rows<T, R, RESID, 32, 512>(s, p)));
+    else if (p.width <= 512) BLH_TRY((launch_bwd_rows<T, R, RESID, 64, 512>(s, p)));
+    else if (p.width <= 1024) BLH_TRY((launch_bwd_rows<T, R, RESID, 128, 512>(s, p)));
+    else if (p.width <= 2048) BLH_TRY((launch_bwd_rows<T, R, RESID, 256, 1024>(s, p)));
+    else if (p.width <= 4096) BLH_TRY((launch_bwd_rows<T, R, RESID, 512, 1024>(s, p)));
+    else BLH_TRY((launch_bwd_rows<T, R, RESID, 1024, 1024>(s, p)));
   } else if (p.rows > 0) {
     if (p.dx || p.dres) {
       const unsigned blocks = (unsigned)std::min<int64_t>(p.rows, 1 << 16);
