@@ -30,6 +30,7 @@ struct NormBwd {
   float* part;          // [chunks][2][stride]: partial column sums of dy hat and dy
   int64_t lddy, lddh, ldh, rows, width, chunk, stride;
   int chunks;
+  int row_blocks;       // few rows: blocks of the launch that take rows, those behind them take columns
   bool same;
   RowDrop drop;
 };
@@ -322,14 +323,58 @@ __global__ __launch_bounds__(BLOCK) void norm_fwd_rows_kernel(NormFwd p) {
   }
 }
 
+// Few rows: dg and db of 64 columns by one block of 512 threads that reads all rows itself (8 lanes of a unit, 64 slices of
+// the rows), so that the backward is one launch without partial sums.
+template <typename T, typename R, bool SHORT>
+__device__ __forceinline__ void norm_few_cols(const NormBwd& p, int block) {
+  __shared__ float sh[8][8][2 * ROW_UNIT];
+  const int lane = threadIdx.x & 7, wave = threadIdx.x >> 6, W = (int)p.width, c0 = block * 64, c = c0 + lane * ROW_UNIT;
+  float a[2 * ROW_UNIT] = {};
+  for (int row = threadIdx.x >> 3; row < (int)p.rows; row += 64) {
+    RawUnit<T> d = load_raw<SHORT>(static_cast<const T*>(p.dy) + row * p.lddy, c, W);
+    const RawUnit<R> f = load_raw<SHORT>(static_cast<const R*>(p.h) + row * p.ldh, c, W);
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    RawUnit<R> h = f;
+    settle(d, c, W);
+    settle(h, c, W);
+#pragma unroll
+    for (int e = 0; e < ROW_UNIT; ++e) {
+      a[e] = fmaf(d.get(e), (h.get(e) - mean) * rstd, a[e]);
+      a[ROW_UNIT + e] += d.get(e);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2 * ROW_UNIT; ++e) {
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) a[e] += __shfl_xor(a[e], o);
+    if ((threadIdx.x & 63) < 8) sh[wave][lane][e] = a[e];
+  }
+  __syncthreads();
+  const int which = threadIdx.x >> 6, j = threadIdx.x & 63;
+  void* out = which ? p.dbeta : p.dgamma;
+  if (which < 2 && out && c0 + j < W) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += sh[w][j / ROW_UNIT][which * ROW_UNIT + j % ROW_UNIT];
+    if (p.same) static_cast<T*>(out)[c0 + j] = (T)v;
+    else static_cast<float*>(out)[c0 + j] = v;
+  }
+}
+
 // partial rows a block of the backward holds in LDS: one for each wave (groups inside a wave join by shuffles) or for each
 // group of waves, but the first, which stays in registers
 template <int LANES, int BLOCK> constexpr int bwd_shares() { return LANES < 64 ? BLOCK / 64 : BLOCK / LANES; }
 
 // One block's rows, a unit a lane: dh' (and dx), and the block's partial column sums in its row of p.part.
-template <typename T, typename R, bool RESID, int LANES, int BLOCK, bool SHORT>
+template <typename T, typename R, bool RESID, int LANES, int BLOCK, bool SHORT, bool FEW>
 __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
   constexpr int GROUPS = BLOCK / LANES, SHARES = bwd_shares<LANES, BLOCK>();
+  if constexpr (FEW) {
+    if ((int)blockIdx.x >= p.row_blocks) {
+      norm_few_cols<T, R, SHORT>(p, blockIdx.x - p.row_blocks);
+      return;
+    }
+  }
   __shared__ float2 sh[2][16];
   extern __shared__ f32x4 cols4[];         // [SHARES - 1][2][stride]
   RowGroup<LANES> group;
@@ -394,7 +439,7 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
     }
     if (p.dx) store_unit(static_cast<T*>(p.dx) + row * p.width, c, width, o);
   }
-  if (!p.part) return;
+  if (FEW || !p.part) return;
   if constexpr (LANES < 64) {
 #pragma unroll
     for (int e = 0; e < ROW_UNIT; ++e)
@@ -436,7 +481,12 @@ static constexpr int64_t ROW_RESIDENT = 8192;      // widest row that stays in r
 // against 72.8; 1024 blocks of 256 threads 73).
 static constexpr int64_t ROW_TWO_BLOCKS = 1024;
 static int norm_blocks(int64_t width) { return width <= ROW_TWO_BLOCKS ? 512 : 256; }
+// One launch without partial sums (norm_few_cols) for few rows.  Kernel time, first launch's start to last one's end, of 64 /
+// 512 / 1024 / 2048 rows of 1024 bf16: 4.3 / 6.3 / 9.1 / 14.1 us, by the two launches 15.8 / 16.3 / 15.1 / 15.2 (2048
+// columns: 4.3 / 6.8 / 10.0 / 22.8 against 15.9 / 15.3 / 16.8 / 16.4).
+static bool norm_few(int64_t rows, int64_t width) { return rows > 0 && rows <= 1024 && width <= 4096; }
 static int norm_partials(int64_t rows, int64_t width) {
+  if (norm_few(rows, width)) return 0;
   return (int)(width <= ROW_RESIDENT ? std::min<int64_t>(rows, norm_blocks(width)) : ceil_div(rows, norm_chunk(rows)));
 }
 
@@ -484,7 +534,17 @@ template <typename T, typename R, bool RESID, int LANES, int BLOCK, bool SHORT =
 static int launch_bwd_rows(hipStream_t s, NormBwd& p) {
   p.chunks = (int)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), norm_blocks(p.width));
   const size_t lds = p.part ? (bwd_shares<LANES, BLOCK>() - 1) * 2 * p.stride * sizeof(float) : 0;    // at most 48 KiB
-  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, BLOCK, SHORT>), dim3((unsigned)p.chunks), dim3(BLOCK), lds, s, p);
+  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, BLOCK, SHORT, false>), dim3((unsigned)p.chunks), dim3(BLOCK), lds, s,
+                     p);
+  BLH_HIP_TRY(hipGetLastError());
+  return BLH_OK;
+}
+
+template <typename T, typename R, bool RESID, int LANES, bool SHORT = false>
+static int launch_bwd_few(hipStream_t s, NormBwd p) {
+  p.row_blocks = p.dx || p.dres ? (int)ceil_div(p.rows, 512 / LANES) : 0;
+  const unsigned blocks = (unsigned)(p.row_blocks + ceil_div(p.width, 64));
+  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, 512, SHORT, true>), dim3(blocks), dim3(512), 0, s, p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
 }
@@ -494,6 +554,14 @@ static int launch_norm_bwd(hipStream_t s, NormBwd p) {
   const bool grads = p.dgamma || p.dbeta;
   p.stride = norm_stride(p.width);
   if (!grads) p.part = nullptr;
+  if (grads && norm_few(p.rows, p.width)) {
+    if (p.width < ROW_UNIT) return launch_bwd_few<T, R, RESID, 16, true>(s, p);
+    if (p.width <= 128) return launch_bwd_few<T, R, RESID, 16>(s, p);
+    if (p.width <= 512) return launch_bwd_few<T, R, RESID, 64>(s, p);
+    if (p.width <= 1024) return launch_bwd_few<T, R, RESID, 128>(s, p);
+    if (p.width <= 2048) return launch_bwd_few<T, R, RESID, 256>(s, p);
+    return launch_bwd_few<T, R, RESID, 512>(s, p);
+  }
   if (p.rows > 0 && p.width <= ROW_RESIDENT) {
     if (p.width < ROW_UNIT) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 512, true>(s, p)));
     else if (p.width <= 128) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 512>(s, p)));
@@ -608,7 +676,7 @@ int blh_residual_norm_forward(void* stream, const void* x, int64_t ldx, const vo
 
 int64_t blh_row_norm_workspace_bytes(int64_t rows, int64_t width) {
   BLH_TRY(row_check_shape(rows, width));
-  return std::max<int64_t>(256, (int64_t)norm_partials(rows, width) * 2 * norm_stride(width) * (int64_t)sizeof(float));
+  return (int64_t)norm_partials(rows, width) * 2 * norm_stride(width) * (int64_t)sizeof(float);
 }
 
 int blh_layer_norm_backward(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
@@ -622,12 +690,11 @@ int blh_layer_norm_backward(void* stream, const void* dy, int64_t lddy, const vo
   if (!row_aligned(dy, dtype) || !row_aligned(x, dtype) || !row_aligned(dx, dtype) || !row_aligned(weight, param_dtype) ||
       !row_aligned(dweight, param_dtype) || !row_aligned(dbias, param_dtype))
     return BLH_ERR_INVALID_ARGUMENT;
-  if (dweight || dbias) {
-    if (!workspace || (uintptr_t)workspace % 16 != 0) return BLH_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < blh_row_norm_workspace_bytes(rows, width)) return BLH_ERR_WORKSPACE;
-  }
+  const int64_t need = dweight || dbias ? blh_row_norm_workspace_bytes(rows, width) : 0;
+  if (need > 0 && (!workspace || (uintptr_t)workspace % 16 != 0)) return BLH_ERR_INVALID_ARGUMENT;
+  if (need > workspace_bytes) return BLH_ERR_WORKSPACE;
   const NormBwd p{dy, nullptr, x, weight, mean, rstd, dx, nullptr, dweight, dbias, static_cast<float*>(workspace),
-                  lddy, 0, ldx, rows, width, 0, 0, 0, param_dtype == dtype, NO_DROP};
+                  lddy, 0, ldx, rows, width, 0, 0, 0, 0, param_dtype == dtype, NO_DROP};
   return norm_bwd((hipStream_t)stream, p, dtype);
 }
 
@@ -647,12 +714,11 @@ int blh_residual_norm_backward(void* stream, const void* dy, int64_t lddy, const
       !row_aligned(h, stream_dtype) || !row_aligned(dresidual, stream_dtype) || !row_aligned(weight, param_dtype) ||
       !row_aligned(dweight, param_dtype) || !row_aligned(dbias, param_dtype))
     return BLH_ERR_INVALID_ARGUMENT;
-  if (dweight || dbias) {
-    if (!workspace || (uintptr_t)workspace % 16 != 0) return BLH_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < blh_row_norm_workspace_bytes(rows, width)) return BLH_ERR_WORKSPACE;
-  }
+  const int64_t need = dweight || dbias ? blh_row_norm_workspace_bytes(rows, width) : 0;
+  if (need > 0 && (!workspace || (uintptr_t)workspace % 16 != 0)) return BLH_ERR_INVALID_ARGUMENT;
+  if (need > workspace_bytes) return BLH_ERR_WORKSPACE;
   const NormBwd p{dy, dh, h, weight, mean, rstd, dx, dresidual, dweight, dbias, static_cast<float*>(workspace),
-                  lddy, lddh, ldh, rows, width, 0, 0, 0, param_dtype == dtype, d};
+                  lddy, lddh, ldh, rows, width, 0, 0, 0, 0, param_dtype == dtype, d};
   return resid_bwd((hipStream_t)stream, p, dtype, stream_dtype);
 }
 

@@ -200,10 +200,26 @@ __device__ __forceinline__ RowKey row_key(const RowDrop& d) {
   return RowKey{(uint32_t)d.seed ^ (uint32_t)(step >> 32), (uint32_t)(d.seed >> 32), d.layer, (uint32_t)step};
 }
 
+// Philox4x32-10 with each round's two products as 32 x 32 -> 64 bit multiplies (one v_mad_u64_u32 each where philox.h's
+// high and low halves are two quarter-rate multiplies: 16384 x 2048 bf16 dropout 22.6 against 23.6 us)
+__device__ __forceinline__ Philox128 philox_row(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c1 = (uint32_t)p1;
+    c3 = (uint32_t)p0;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return Philox128{{c0, c1, c2, c3}};
+}
+
 // the 16-bit draws of the unit at columns 8 unit .. 8 unit + 7 of global row `row`: an element is kept where
 // its draw reaches the threshold
 __device__ __forceinline__ void draw_unit(const RowKey& k, int64_t row, int64_t unit, uint32_t (&u)[ROW_UNIT]) {
-  const Philox128 q = philox4x32_10((uint32_t)row, (uint32_t)unit | ((uint32_t)(row >> 32) << 21), k.c2, k.c3, k.k0, k.k1);
+  const Philox128 q = philox_row((uint32_t)row, (uint32_t)unit | ((uint32_t)(row >> 32) << 21), k.c2, k.c3, k.k0, k.k1);
 #pragma unroll
   for (int e = 0; e < ROW_UNIT; ++e) u[e] = (e & 1) ? q.w[e >> 1] >> 16 : q.w[e >> 1] & 0xFFFFu;
 }

@@ -179,7 +179,7 @@ struct ParamGrads {
     if (need_weight || need_bias) {
       const int64_t need = blh_row_norm_workspace_bytes(rows_of(x), x.size(-1));
       if (need < 0) check_status((int)need, "blh_row_norm_workspace_bytes");
-      workspace = at::empty({need}, x.options().dtype(at::kByte));
+      if (need > 0) workspace = at::empty({need}, x.options().dtype(at::kByte));
     }
   }
   int64_t bytes() const { return workspace.defined() ? workspace.numel() : 0; }

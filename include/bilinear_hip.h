@@ -523,8 +523,8 @@ int blh_row_dropout(void* stream, const void* x, int64_t ldx, void* y, const blh
 int blh_layer_norm_forward(void* stream, const void* x, int64_t ldx, const void* weight, const void* bias, double eps,
                            void* y, float* mean, float* rstd, int64_t rows, int64_t width, int32_t dtype,
                            int32_t param_dtype);
-/* dx, dweight, dbias: each may be NULL (not computed).  `workspace` (blh_row_norm_workspace_bytes, 16-byte aligned) is
- * needed for dweight / dbias; its contents mean nothing between calls.                                               */
+/* dx, dweight, dbias: each may be NULL (not computed).  `workspace` (blh_row_norm_workspace_bytes, 16-byte aligned; 0
+ * bytes for few rows) is needed for dweight / dbias; its contents mean nothing between calls.                        */
 int64_t blh_row_norm_workspace_bytes(int64_t rows, int64_t width);
 int blh_layer_norm_backward(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
                             const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
