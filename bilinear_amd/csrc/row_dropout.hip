@@ -14,7 +14,9 @@
 namespace blh {
 
 int row_make_drop(const blh_row_drop* d, int64_t rows, RowDrop* out) {
-  if (!(d->p >= 0.0 && d->p <= 1.0) || d->layer < 0 || d->row_offset < 0) return BLH_ERR_INVALID_ARGUMENT;
+  if (!(d->p >= 0.0 && d->p <= 1.0) || d->layer < 0 || d->row_offset < 0 ||
+      (d->step_used && d->step_used == d->step_dev))
+    return BLH_ERR_INVALID_ARGUMENT;
   if (d->row_offset > ROW_MAX_ROWS - rows) return BLH_ERR_SHAPE;
   const uint32_t t = (uint32_t)(d->p * 65536.0 + 0.5);
   *out = RowDrop{d->seed, d->step, d->step_dev, d->step_used, d->row_offset, (uint32_t)d->layer | 0x80000000u, t,

@@ -234,7 +234,6 @@ class _Draws:
             raise RuntimeError("the device step is one int64")
         self._device_step = tensor
 
-    @torch.compiler.disable
     def _next_draws(self):
         if self._seed is None:
             self._seed = int(torch.initial_seed()) & ((1 << 63) - 1)

@@ -511,6 +511,47 @@ def test_under_torch_compile(B):
         assert torch.equal(p, q)
 
 
+def test_compiled_functions_of_one_output_and_compiled_modules(B):
+    x, r = data(40, 96, F32, 1).requires_grad_(), data(40, 96, F32, 2).requires_grad_()
+    dh = data(40, 96, F32, 4)
+    f = lambda x, r: B.residual_norm(x, r, p=0.2, seed=5)[1]     # noqa: E731
+    want = torch.autograd.grad(f(x, r), (x, r), dh)
+    for p, q in zip(torch.autograd.grad(torch.compile(f, backend="aot_eager", fullgraph=True)(x, r), (x, r), dh), want):
+        assert torch.equal(p, q)
+    net = torch.nn.Sequential(B.LayerNorm(96), B.Dropout(0.3)).cuda()
+    step = torch.compile(net, backend="aot_eager")
+    outs = []
+    for compiled in (False, True):
+        torch.manual_seed(21)
+        outs.append([(step if compiled else net)(x) for _ in range(4)])
+    for p, q in zip(*outs):
+        assert torch.equal(p, q)
+    assert not torch.equal(outs[0][0], outs[0][1])
+
+
+def test_offsets_past_32_bits(B):
+    """More than 2^32 elements: the last rows are those of the same rows on their own (bit for bit: rows do not meet)."""
+    rows, width = (1 << 19) + 3, 8192
+    w, b = params(width, F32, 5)
+    block = data(1024, width, BF16, 1)
+    x = torch.empty(rows, width, dtype=BF16, device="cuda")
+    for i in range(0, rows, 1024):
+        x[i:i + 1024] = block[:min(1024, rows - i)]
+    x.requires_grad_()
+    tail = x.detach()[-5:].clone().requires_grad_()
+    y, small = B.layer_norm(x, w, b), B.layer_norm(tail, w, b)
+    assert torch.equal(y[-5:], small)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    assert torch.equal(dx[-5:], torch.autograd.grad(small, tail, tail.detach())[0])
+    del y, dx
+    y = B.dropout(x.detach(), 0.3, seed=3)
+    assert torch.equal(y[-5:], B.dropout(tail.detach(), 0.3, seed=3, row_offset=rows - 5))
+    del y
+    y, h = B.residual_norm(x.detach(), x.detach(), p=0.3, seed=3)
+    u, v = B.residual_norm(tail.detach(), tail.detach(), p=0.3, seed=3, row_offset=rows - 5)
+    assert torch.equal(y[-5:], u) and torch.equal(h[-5:], v)
+
+
 def test_the_custom_operators_refuse_what_the_functions_refuse(B):
     x = torch.zeros(2, 8, device="cuda")
     op = torch.ops.bilinear_hip

@@ -57,6 +57,8 @@ def test_c_abi_refuses_bad_arguments(native):
     for p in (-0.1, 1.1, float("nan")):
         assert drop(None, at, 8, at, _drop(p=p), 2, 8, 0) == -1
     assert drop(None, None, 8, at, _drop(), 2, 8, 0) == -1
+    same = N.RowDrop(0.1, 1, 0, 0, at, at, 0, 0)                               # the step read is the step written
+    assert drop(None, at, 8, at, ctypes.byref(same), 2, 8, 0) == -1
     assert drop(None, at + 2, 8, at, _drop(), 2, 8, 0) == -1                   # fp32 off its alignment
     assert drop(None, at + 1, 8, at, _drop(), 2, 8, 1) == -1
     assert drop(None, None, 8, None, _drop(), 0, 8, 0) == 0                    # no rows: nothing to do
