@@ -475,7 +475,7 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
 // rows of one partial sum of the wide form: whole groups of 16 rows, at most 256 chunks
 static int64_t norm_chunk(int64_t rows) { return round_up(std::max<int64_t>(1, ceil_div(rows, 256)), 16); }
 static int64_t norm_stride(int64_t width) { return round_up(width, ROW_UNIT); }
-static constexpr int64_t ROW_RESIDENT = 8192;      // widest row that stays in registers
+static constexpr int64_t ROW_RESIDENT = 8192;      // widest row that stays in the backward's registers (the forward: 16384)
 // Blocks of the resident backward: 16 waves a CU, in two blocks of 512 threads, or in one of 1024 where a row is over 1024
 // columns and its partial sums are the larger cost (16384 x 2048 bf16 residual norm 65.3 against 68.4 us, 8192 x 4096 67.2
 // against 72.8; 1024 blocks of 256 threads 73).
@@ -510,7 +510,8 @@ template <typename T, typename R, bool RESID>
 static int launch_norm_fwd(hipStream_t s, const NormFwd& p) {
   constexpr bool wide = sizeof(T) == 4;
   const bool few = p.rows <= 2048;
-  if (p.width < ROW_UNIT) return launch_fwd_rows<T, R, RESID, 16, 1, true>(s, p);
+  if (p.width < ROW_UNIT) return launch_fwd_rows<T, R, RESID, 8, 1, true>(s, p);
+  if (p.width <= 64) return launch_fwd_rows<T, R, RESID, 8, 1>(s, p);
   if (p.width <= 128) return launch_fwd_rows<T, R, RESID, 16, 1>(s, p);
   if (p.width <= 256) return launch_fwd_rows<T, R, RESID, 32, 1>(s, p);
   if (p.width <= 512) return launch_fwd_rows<T, R, RESID, 64, 1>(s, p);
@@ -523,7 +524,8 @@ static int launch_norm_fwd(hipStream_t s, const NormFwd& p) {
     if constexpr (!wide) return launch_fwd_rows<T, R, RESID, RESID ? 128 : 64, RESID ? 2 : 4>(s, p);
   }
   if (p.width <= 4096) return launch_fwd_rows<T, R, RESID, wide ? 512 : 256, wide ? 1 : 2>(s, p);
-  if (p.width <= ROW_RESIDENT) return launch_fwd_rows<T, R, RESID, wide ? 512 : 256, wide ? 2 : 4>(s, p);
+  if (p.width <= 8192) return launch_fwd_rows<T, R, RESID, wide ? 512 : 256, wide ? 2 : 4>(s, p);
+  if (p.width <= 16384) return launch_fwd_rows<T, R, RESID, 1024, 2>(s, p);
   const unsigned blocks = (unsigned)std::min<int64_t>(p.rows, 1 << 16);
   hipLaunchKernelGGL((norm_fwd_kernel<T, R, RESID>), dim3(blocks), dim3(256), 0, s, p);
   BLH_HIP_TRY(hipGetLastError());
@@ -555,7 +557,8 @@ static int launch_norm_bwd(hipStream_t s, NormBwd p) {
   p.stride = norm_stride(p.width);
   if (!grads) p.part = nullptr;
   if (grads && norm_few(p.rows, p.width)) {
-    if (p.width < ROW_UNIT) return launch_bwd_few<T, R, RESID, 16, true>(s, p);
+    if (p.width < ROW_UNIT) return launch_bwd_few<T, R, RESID, 8, true>(s, p);
+    if (p.width <= 64) return launch_bwd_few<T, R, RESID, 8>(s, p);
     if (p.width <= 128) return launch_bwd_few<T, R, RESID, 16>(s, p);
     if (p.width <= 512) return launch_bwd_few<T, R, RESID, 64>(s, p);
     if (p.width <= 1024) return launch_bwd_few<T, R, RESID, 128>(s, p);
@@ -563,7 +566,8 @@ static int launch_norm_bwd(hipStream_t s, NormBwd p) {
     return launch_bwd_few<T, R, RESID, 512>(s, p);
   }
   if (p.rows > 0 && p.width <= ROW_RESIDENT) {
-    if (p.width < ROW_UNIT) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 512, true>(s, p)));
+    if (p.width < ROW_UNIT) BLH_TRY((launch_bwd_rows<T, R, RESID, 8, 512, true>(s, p)));
+    else if (p.width <= 64) BLH_TRY((launch_bwd_rows<T, R, RESID, 8, 512>(s, p)));
     else if (p.width <= 128) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 512>(s, p)));
     else if (p.width <= 256) BLH_TRY((launch_bwd_rows<T, R, RESID, 32, 512>(s, p)));
     else if (p.width <= 512) BLH_TRY((launch_bwd_rows<T, R, RESID, 64, 512>(s, p)));

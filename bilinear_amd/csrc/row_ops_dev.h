@@ -164,11 +164,16 @@ template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ float dpp_add(flo
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
 }
 
-// sum over groups of LANES consecutive lanes (16, 32 or 64), in every lane; all 64 lanes take part.  Rotations inside
-// rows of 16 lanes pair equal partial sums, so a group's lanes agree bit for bit; whole waves join their rows by the two
-// row broadcasts and read the last lane.
+// sum over groups of LANES consecutive lanes (8, 16, 32 or 64), in every lane; all 64 lanes take part.  Each step pairs
+// lanes that hold the same partial sum's two halves, so a group's lanes agree bit for bit; whole waves join their rows of 16
+// by the two row broadcasts and read the last lane.
 template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
-  v = dpp_add<0x128>(v);       // row_ror:8, 4, 2, 1
+  if constexpr (LANES == 8) {
+    v = dpp_add<0xB1>(v);        // quad_perm 1 0 3 2
+    v = dpp_add<0x4E>(v);        // quad_perm 2 3 0 1
+    return dpp_add<0x141>(v);    // row_half_mirror: the other quad
+  }
+  v = dpp_add<0x128>(v);         // row_ror:8, 4, 2, 1
   v = dpp_add<0x124>(v);
   v = dpp_add<0x122>(v);
   v = dpp_add<0x121>(v);
