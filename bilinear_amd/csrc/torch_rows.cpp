@@ -105,12 +105,16 @@ void check_status(int status, const char* what) {
 
 // ---- native calls (checked tensors) ---------------------------------------------------------------------------------
 
+// What a kernel may read: a lazily negated view (an imaginary part of a conjugate) is resolved first.
+Tensor readable(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // Rows are read in place where the last axis is dense and the leading axes collapse to one, else from a dense copy.
 struct Rows {
   Tensor t;
   int64_t ld;
   Rows() : ld(0) {}
-  explicit Rows(const Tensor& x) : t(x), ld(x.size(-1)) {
+  explicit Rows(const Tensor& given) : t(readable(given)), ld(given.size(-1)) {
+    const Tensor x = t;
     if (x.is_contiguous()) return;
     const int64_t width = x.size(-1), n = x.dim();
     if (x.stride(-1) == 1 || width == 1) {
@@ -132,7 +136,7 @@ struct Rows {
   const void* ptr() const { return t.defined() ? t.const_data_ptr() : nullptr; }
 };
 
-Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor dense(const Tensor& t) { return t.defined() ? readable(t).contiguous() : t; }
 Tensor plain(const Optional& t) { return t ? *t : Tensor(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -332,6 +336,9 @@ template <typename N> std::shared_ptr<N> make_node() {
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                "bilinear_amd row operators have no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : inputs)
     if (t->defined() && t->requires_grad()) return true;

@@ -226,6 +226,30 @@ def test_a_second_thread_and_single_threaded_backward(B):
             assert torch.equal(p, q)
 
 
+def test_lazily_negated_views_and_forward_mode(B):
+    z = torch.view_as_complex(data(6, 80, F32, 1).view(6, 40, 2))
+    x = z.conj().imag                        # a float view that is to be read negated
+    assert x.is_neg()
+    w, b = params(40, F32, 5)
+    assert torch.equal(B.layer_norm(x, w, b), B.layer_norm(x.resolve_neg(), w, b))
+    assert torch.equal(B.dropout(x, 0.5, seed=1), B.dropout(x.resolve_neg(), 0.5, seed=1))
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        dual = fwd.make_dual(data(3, 8, F32, 1), data(3, 8, F32, 2))
+        with pytest.raises(NotImplementedError):
+            B.layer_norm(dual)
+
+
+def test_custom_operators_are_what_their_schemas_say(B):
+    x, r = data(6, 40, BF16, 1).requires_grad_(), data(6, 40, F32, 2).requires_grad_()
+    w, b = params(40, F32, 5)
+    op = torch.ops.bilinear_hip
+    checks = ("test_schema", "test_autograd_registration", "test_faketensor")
+    torch.library.opcheck(op.layer_norm.default, (x, w, b, 1e-5), test_utils=checks)
+    torch.library.opcheck(op.row_dropout.default, (x, 0.3, 1, 2, 3, 4, None), test_utils=checks)
+    torch.library.opcheck(op.residual_norm.default, (x, r, w, b, 1e-5, 0.3, 1, 2, 3, 4, None), test_utils=checks)
+
+
 def test_double_backward_is_refused(B):
     x = data(3, 16, F32, 1).requires_grad_()
     g, = torch.autograd.grad(B.layer_norm(x).square().sum(), x, create_graph=True)
