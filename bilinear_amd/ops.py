@@ -12,6 +12,8 @@ the C ABI directly, since a callback has no operator-schema type.
     torch.ops.bilinear_hip.backward(x, dpred, params, workspace, grads, masks, ...)
     pred, loss = torch.ops.bilinear_hip.train_step(x, target, params, grads, exp_avg, ...)
 
+The row operators (layer_norm, row_dropout, residual_norm and their backward operators) are registered by row_ops.py.
+
 Reference call-sites: BilinearUnit.forward (/root/reference/model/bilinear.py:31-41, eval:
 valid_bilinear.py:31,52), loss.backward() (train_bilinear.py:79), the step body
 (train_bilinear.py:75-83).  ``ctx`` is the integer value of a ``blh_context*`` (bilinear_amd.
