@@ -45,7 +45,7 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
 }
 
 // ---- rows that are read again in each pass: any width ---------------------------------------------------------------------
-// (over 16384 columns forward, over 8192 backward; 1024 x 16384 bf16: backward 48 us = 2.1 TB/s of its bytes)
+// (over 16384 columns; 512 x 32768 bf16: layer norm forward 24 us = 2.8 TB/s of its bytes, backward 51 us = 2.0)
 
 template <typename T, typename R, bool RESID>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormFwd p) {
@@ -369,8 +369,9 @@ __device__ __forceinline__ void norm_few_cols(const NormBwd& p, int block) {
 // group of waves, but the first, which stays in registers
 template <int LANES, int BLOCK> constexpr int bwd_shares() { return LANES < 64 ? BLOCK / 64 : BLOCK / LANES; }
 
-// One block's rows, a unit a lane: dh' (and dx), and the block's partial column sums in its row of p.part.
-template <typename T, typename R, bool RESID, int LANES, int BLOCK, bool SHORT, bool FEW>
+// One block's rows, NV units a lane (one; two in rows of over 8192 columns: 1024 x 16384 bf16 33 us, read again in each pass
+// 48): dh' (and dx), and the block's partial column sums in its row of p.part.
+template <typename T, typename R, bool RESID, int LANES, int NV, int BLOCK, bool SHORT, bool FEW>
 __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
   constexpr int GROUPS = BLOCK / LANES, SHARES = bwd_shares<LANES, BLOCK>();
   if constexpr (FEW) {
@@ -383,23 +384,32 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
   extern __shared__ f32x4 cols4[];         // [SHARES - 1][2][stride]
   RowGroup<LANES> group;
   const RowKey key = RESID && p.drop.threshold ? row_key(p.drop) : RowKey{};
-  const int W = (int)p.width, u = threadIdx.x % LANES, c = u * ROW_UNIT;
+  const int W = (int)p.width, lane = threadIdx.x % LANES;
   int g = threadIdx.x / LANES;
   if constexpr (LANES == 64) g = __builtin_amdgcn_readfirstlane(g);
-  float gm[ROW_UNIT], ag[ROW_UNIT] = {}, ab[ROW_UNIT] = {};
-  load_param_unit<SHORT, T>(p.gamma, p.same, c, W, 1.f, gm);
-  struct In { RawUnit<T> d; RawUnit<R> f, dh; float mean, rstd; };
+  float gm[NV][ROW_UNIT], ag[NV][ROW_UNIT], ab[NV][ROW_UNIT];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_param_unit<SHORT, T>(p.gamma, p.same, (i * LANES + lane) * ROW_UNIT, W, 1.f, gm[i]);
+#pragma unroll
+    for (int e = 0; e < ROW_UNIT; ++e) ag[i][e] = ab[i][e] = 0.f;
+  }
+  struct In { RawUnit<T> d[NV]; RawUnit<R> f[NV], dh[NV]; float mean, rstd; };
   auto load = [&](int64_t row, In& q) {
     row = min(row, p.rows - 1);                    // (a group behind the last row reads that one and writes nothing)
-    q.d = load_raw<SHORT>(static_cast<const T*>(p.dy) + row * p.lddy, c, W);
-    q.f = load_raw<SHORT>(static_cast<const R*>(p.h) + row * p.ldh, c, W);
-    if (RESID && p.dh) q.dh = load_raw<SHORT>(static_cast<const R*>(p.dh) + row * p.lddh, c, W);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * ROW_UNIT;
+      q.d[i] = load_raw<SHORT>(static_cast<const T*>(p.dy) + row * p.lddy, c, W);
+      q.f[i] = load_raw<SHORT>(static_cast<const R*>(p.h) + row * p.ldh, c, W);
+      if (RESID && p.dh) q.dh[i] = load_raw<SHORT>(static_cast<const R*>(p.dh) + row * p.lddh, c, W);
+    }
     q.mean = p.mean[row];
     q.rstd = p.rstd[row];
   };
   // the next row's loads go out in front of this row's sums where that costs at most 12 registers (16384 x 1024 bf16: 21.9
   // against 22.9 us; with an fp32 stream the registers cost more waves than the loads bring: 8192 x 1024 36.3 against 35.2)
-  constexpr bool AHEAD = sizeof(T) + (RESID ? 2 : 1) * sizeof(R) <= 6;
+  constexpr bool AHEAD = NV * (sizeof(T) + (RESID ? 2 : 1) * sizeof(R)) <= 6;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   In next;
   if constexpr (AHEAD) load((int64_t)blockIdx.x * GROUPS + g, next);
@@ -413,65 +423,78 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
     } else {
       load(row, in);
     }
-    settle(in.d, c, width);                        // (dy is 0 behind the row's end)
-    settle(in.f, c, width);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int e = 0; e < ROW_UNIT; ++e) {
-      const float v = in.d.get(e), hat = (in.f.get(e) - in.mean) * in.rstd, t = v * gm[e];
-      s1 += t;
-      s2 = fmaf(t, hat, s2);
-      ag[e] = fmaf(v, hat, ag[e]);
-      ab[e] += v;
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * ROW_UNIT;
+      settle(in.d[i], c, width);                   // (dy is 0 behind the row's end)
+      settle(in.f[i], c, width);
+#pragma unroll
+      for (int e = 0; e < ROW_UNIT; ++e) {
+        const float v = in.d[i].get(e), hat = (in.f[i].get(e) - in.mean) * in.rstd, t = v * gm[i][e];
+        s1 += t;
+        s2 = fmaf(t, hat, s2);
+        ag[i][e] = fmaf(v, hat, ag[i][e]);
+        ab[i][e] += v;
+      }
     }
     group.sum2(s1, s2, sh);
     const float c1 = s1 / (float)W, c2 = s2 / (float)W;
-    float o[ROW_UNIT];
 #pragma unroll
-    for (int e = 0; e < ROW_UNIT; ++e) {
-      const float hat = (in.f.get(e) - in.mean) * in.rstd;
-      o[e] = in.rstd * (fmaf(in.d.get(e), gm[e], -c1) - hat * c2);
-    }
-    if constexpr (RESID) {
-      if (p.dh) {
-        settle(in.dh, c, width);
+    for (int i = 0; i < NV; ++i) {
+      const int u = i * LANES + lane, c = u * ROW_UNIT;
+      float o[ROW_UNIT];
 #pragma unroll
-        for (int e = 0; e < ROW_UNIT; ++e) o[e] += in.dh.get(e);
+      for (int e = 0; e < ROW_UNIT; ++e) {
+        const float hat = (in.f[i].get(e) - in.mean) * in.rstd;
+        o[e] = in.rstd * (fmaf(in.d[i].get(e), gm[i][e], -c1) - hat * c2);
       }
-      if (p.dres) store_unit(static_cast<R*>(p.dres) + row * p.width, c, width, o);
-      if (p.dx && p.drop.threshold) drop_unit(key, p.drop, p.drop.row_offset + row, u, o);
+      if constexpr (RESID) {
+        if (p.dh) {
+          settle(in.dh[i], c, width);
+#pragma unroll
+          for (int e = 0; e < ROW_UNIT; ++e) o[e] += in.dh[i].get(e);
+        }
+        if (p.dres) store_unit(static_cast<R*>(p.dres) + row * p.width, c, width, o);
+        if (p.dx && p.drop.threshold) drop_unit(key, p.drop, p.drop.row_offset + row, u, o);
+      }
+      if (p.dx) store_unit(static_cast<T*>(p.dx) + row * p.width, c, width, o);
     }
-    if (p.dx) store_unit(static_cast<T*>(p.dx) + row * p.width, c, width, o);
   }
   if (FEW || !p.part) return;
-  if constexpr (LANES < 64) {
-#pragma unroll
-    for (int e = 0; e < ROW_UNIT; ++e)
-#pragma unroll
-      for (int o = LANES; o < 64; o <<= 1) {
-        ag[e] += __shfl_xor(ag[e], o);
-        ab[e] += __shfl_xor(ab[e], o);
-      }
-  }
   const int share = LANES < 64 ? threadIdx.x >> 6 : threadIdx.x / LANES;
-  const bool mine = (LANES >= 64 || (threadIdx.x & 63) < LANES) && c < W;
-  f32x4 a[4] = {{ag[0], ag[1], ag[2], ag[3]}, {ag[4], ag[5], ag[6], ag[7]},
-                {ab[0], ab[1], ab[2], ab[3]}, {ab[4], ab[5], ab[6], ab[7]}};
-  const int64_t at[4] = {c / 4, c / 4 + 1, (p.stride + c) / 4, (p.stride + c) / 4 + 1};
-  if constexpr (SHARES > 1) {
-    if (mine && share > 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) cols4[(share - 1) * (p.stride / 2) + at[i]] = a[i];
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + lane) * ROW_UNIT;
+    if constexpr (LANES < 64) {
+#pragma unroll
+      for (int e = 0; e < ROW_UNIT; ++e)
+#pragma unroll
+        for (int o = LANES; o < 64; o <<= 1) {
+          ag[i][e] += __shfl_xor(ag[i][e], o);
+          ab[i][e] += __shfl_xor(ab[i][e], o);
+        }
     }
-    __syncthreads();
-  }
-  if (mine && share == 0) {
-    f32x4* out = reinterpret_cast<f32x4*>(p.part + (int64_t)blockIdx.x * 2 * p.stride);
+    const bool mine = (LANES >= 64 || (threadIdx.x & 63) < LANES) && c < W;
+    f32x4 a[4] = {{ag[i][0], ag[i][1], ag[i][2], ag[i][3]}, {ag[i][4], ag[i][5], ag[i][6], ag[i][7]},
+                  {ab[i][0], ab[i][1], ab[i][2], ab[i][3]}, {ab[i][4], ab[i][5], ab[i][6], ab[i][7]}};
+    const int64_t at[4] = {c / 4, c / 4 + 1, (p.stride + c) / 4, (p.stride + c) / 4 + 1};
+    if constexpr (SHARES > 1) {
+      static_assert(NV == 1 || SHARES == 1, "one unit a lane where shares meet in LDS");
+      if (mine && share > 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+        for (int k = 0; k < 4; ++k) cols4[(share - 1) * (p.stride / 2) + at[k]] = a[k];
+      }
+      __syncthreads();
+    }
+    if (mine && share == 0) {
+      f32x4* out = reinterpret_cast<f32x4*>(p.part + (int64_t)blockIdx.x * 2 * p.stride);
 #pragma unroll
-      for (int k = 1; k < SHARES; ++k) a[i] += cols4[(k - 1) * (p.stride / 2) + at[i]];
-      out[at[i]] = a[i];
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int n = 1; n < SHARES; ++n) a[k] += cols4[(n - 1) * (p.stride / 2) + at[k]];
+        out[at[k]] = a[k];
+      }
     }
   }
 }
@@ -479,7 +502,7 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
 // rows of one partial sum of the wide form: whole groups of 16 rows, at most 256 chunks
 static int64_t norm_chunk(int64_t rows) { return round_up(std::max<int64_t>(1, ceil_div(rows, 256)), 16); }
 static int64_t norm_stride(int64_t width) { return round_up(width, ROW_UNIT); }
-static constexpr int64_t ROW_RESIDENT = 8192;      // widest row that stays in the backward's registers (the forward: 16384)
+static constexpr int64_t ROW_RESIDENT = 16384;     // widest row that stays in registers
 // Blocks of the resident backward: 16 waves a CU, in two blocks of 512 threads, or in one of 1024 where a row is over 1024
 // columns and its partial sums are the larger cost (16384 x 2048 bf16 residual norm 65.3 against 68.4 us, 8192 x 4096 67.2
 // against 72.8; 1024 blocks of 256 threads 73).
@@ -529,18 +552,18 @@ static int launch_norm_fwd(hipStream_t s, const NormFwd& p) {
   }
   if (p.width <= 4096) return launch_fwd_rows<T, R, RESID, wide ? 512 : 256, wide ? 1 : 2>(s, p);
   if (p.width <= 8192) return launch_fwd_rows<T, R, RESID, wide ? 512 : 256, wide ? 2 : 4>(s, p);
-  if (p.width <= 16384) return launch_fwd_rows<T, R, RESID, 1024, 2>(s, p);
+  if (p.width <= ROW_RESIDENT) return launch_fwd_rows<T, R, RESID, 1024, 2>(s, p);
   const unsigned blocks = (unsigned)std::min<int64_t>(p.rows, 1 << 16);
   hipLaunchKernelGGL((norm_fwd_kernel<T, R, RESID>), dim3(blocks), dim3(256), 0, s, p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
 }
 
-template <typename T, typename R, bool RESID, int LANES, int BLOCK, bool SHORT = false>
+template <typename T, typename R, bool RESID, int LANES, int NV, int BLOCK, bool SHORT = false>
 static int launch_bwd_rows(hipStream_t s, NormBwd& p) {
   p.chunks = (int)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), norm_blocks(p.width));
   const size_t lds = p.part ? (bwd_shares<LANES, BLOCK>() - 1) * 2 * p.stride * sizeof(float) : 0;    // at most 48 KiB
-  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, BLOCK, SHORT, false>), dim3((unsigned)p.chunks), dim3(BLOCK), lds, s,
+  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, NV, BLOCK, SHORT, false>), dim3((unsigned)p.chunks), dim3(BLOCK), lds, s,
                      p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
@@ -550,7 +573,7 @@ template <typename T, typename R, bool RESID, int LANES, bool SHORT = false>
 static int launch_bwd_few(hipStream_t s, NormBwd p) {
   p.row_blocks = p.dx || p.dres ? (int)ceil_div(p.rows, 512 / LANES) : 0;
   const unsigned blocks = (unsigned)(p.row_blocks + ceil_div(p.width, 64));
-  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, 512, SHORT, true>), dim3(blocks), dim3(512), 0, s, p);
+  hipLaunchKernelGGL((norm_bwd_kernel<T, R, RESID, LANES, 1, 512, SHORT, true>), dim3(blocks), dim3(512), 0, s, p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;
 }
@@ -570,15 +593,16 @@ static int launch_norm_bwd(hipStream_t s, NormBwd p) {
     return launch_bwd_few<T, R, RESID, 512>(s, p);
   }
   if (p.rows > 0 && p.width <= ROW_RESIDENT) {
-    if (p.width < ROW_UNIT) BLH_TRY((launch_bwd_rows<T, R, RESID, 8, 512, true>(s, p)));
-    else if (p.width <= 64) BLH_TRY((launch_bwd_rows<T, R, RESID, 8, 512>(s, p)));
-    else if (p.width <= 128) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 512>(s, p)));
-    else if (p.width <= 256) BLH_TRY((launch_bwd_rows<T, R, RESID, 32, 512>(s, p)));
-    else if (p.width <= 512) BLH_TRY((launch_bwd_rows<T, R, RESID, 64, 512>(s, p)));
-    else if (p.width <= 1024) BLH_TRY((launch_bwd_rows<T, R, RESID, 128, 512>(s, p)));
-    else if (p.width <= 2048) BLH_TRY((launch_bwd_rows<T, R, RESID, 256, 1024>(s, p)));
-    else if (p.width <= 4096) BLH_TRY((launch_bwd_rows<T, R, RESID, 512, 1024>(s, p)));
-    else BLH_TRY((launch_bwd_rows<T, R, RESID, 1024, 1024>(s, p)));
+    if (p.width < ROW_UNIT) BLH_TRY((launch_bwd_rows<T, R, RESID, 8, 1, 512, true>(s, p)));
+    else if (p.width <= 64) BLH_TRY((launch_bwd_rows<T, R, RESID, 8, 1, 512>(s, p)));
+    else if (p.width <= 128) BLH_TRY((launch_bwd_rows<T, R, RESID, 16, 1, 512>(s, p)));
+    else if (p.width <= 256) BLH_TRY((launch_bwd_rows<T, R, RESID, 32, 1, 512>(s, p)));
+    else if (p.width <= 512) BLH_TRY((launch_bwd_rows<T, R, RESID, 64, 1, 512>(s, p)));
+    else if (p.width <= 1024) BLH_TRY((launch_bwd_rows<T, R, RESID, 128, 1, 512>(s, p)));
+    else if (p.width <= 2048) BLH_TRY((launch_bwd_rows<T, R, RESID, 256, 1, 1024>(s, p)));
+    else if (p.width <= 4096) BLH_TRY((launch_bwd_rows<T, R, RESID, 512, 1, 1024>(s, p)));
+    else if (p.width <= 8192) BLH_TRY((launch_bwd_rows<T, R, RESID, 1024, 1, 1024>(s, p)));
+    else BLH_TRY((launch_bwd_rows<T, R, RESID, 1024, 2, 1024>(s, p)));
   } else if (p.rows > 0) {
     if (p.dx || p.dres) {
       const unsigned blocks = (unsigned)std::min<int64_t>(p.rows, 1 << 16);

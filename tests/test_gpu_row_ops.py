@@ -15,7 +15,7 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 SIZES = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 65), (70, 128), (4, 129), (64, 1024), (37, 333), (1, 512), (9, 513), (4, 2048),
          (3, 2049), (2, 4100), (2, 8192), (3, 8200), (2, 12001), (2, 16384), (2, 16385), (2, 20001), (1, 100003), (300000, 1), (70000, 3), (1030, 48), (2500, 96), (1500, 1000), (1100, 2056),
          # rows on both sides of the one-launch backward (1024), for each of the other's variants
-         (1024, 40), (1025, 40), (1100, 5), (1025, 200), (1100, 400), (1030, 2048), (1025, 2500), (1027, 4100)]
+         (1024, 40), (1025, 40), (1100, 5), (1025, 200), (1100, 400), (1030, 2048), (1025, 2500), (1027, 4100), (300, 9001)]
 
 
 @pytest.fixture(scope="module")
