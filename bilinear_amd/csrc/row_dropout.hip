@@ -8,6 +8,10 @@
 // The mask depends on (seed, step, layer, global row, column) alone: not on the type, the launch or how rows are spread
 // over devices.  p is rounded to a multiple of 2^-16 and s is the exact inverse of the rounded keep probability, so the
 // expectation of y is x.  The backward pass is the same map on dy: there is nothing to save.
+//
+// Bound by memory: 16384 x 2048 bf16 22.6 us = 5.9 TB/s of its bytes on three inputs in turn, 27 us = 5.0 where forward and
+// backward alternate on 800 MB (a copy of 537 MB: 5.0); a stored mask of one bit would add 6 % of the bytes each way.  16 bits
+// a draw make it 1/8 call an element: 32 bits, 1/4 call, would cost a 16-bit type more arithmetic than its bytes take.
 #include "row_ops.h"
 #include "row_ops_dev.h"
 
@@ -24,7 +28,8 @@ int row_make_drop(const blh_row_drop* d, int64_t rows, RowDrop* out) {
   return BLH_OK;
 }
 
-// I: the type that counts units (32 bits wherever they fit: the division by `units` is what the index costs)
+// I: the type that counts units: 32 bits wherever they fit, since the index costs a division by `units` (65536 x 64 bf16 5.4
+// against 5.8 us)
 template <typename T, typename I, bool SHORT>
 __global__ __launch_bounds__(256) void row_dropout_kernel(const T* x, int64_t ldx, T* y, RowDrop drop, I total, I units,
                                                           int width) {

@@ -179,7 +179,8 @@ __global__ __launch_bounds__(256) void norm_bwd_cols_kernel(NormBwd p) {
 }
 
 // dgamma, dbeta = sums of the chunks' partials, in the parameters' type (chunks == 0: zeros).  A block owns 32 columns:
-// 8 lanes x 4 columns, 128 slices of the chunks, so that 512 partial rows are one round trip of four loads.
+// 8 lanes x 4 columns, 128 slices of the chunks, so that 512 partial rows are one round trip of four loads (4 us for 512 rows
+// of 1024 or 256 of 2048 columns: a launch and that round trip).
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_bwd_finish_kernel(NormBwd p) {
   __shared__ f32x4 sh[128][8];

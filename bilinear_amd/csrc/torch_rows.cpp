@@ -3,8 +3,8 @@
 //
 // Why C++ and not ctypes as the lifter's path: these calls are short — at a few hundred rows the kernels take 5-10 us —
 // and autograd runs a backward node on its device thread, where a Python node starts with cold caches.  Measured with
-// ctypes and a Python autograd.Function: forward + backward of a 64 x 1024 layer norm 143 us, of which the kernels are
-// 15; without a gradient 12.6 us.
+// ctypes and a Python autograd.Function: forward + backward of a 64 x 1024 layer norm 143 us, without a gradient 12.6; with
+// these nodes 40-64 us (23.6 with single-threaded autograd; the kernels are 8) and 4.3-5.
 #include <ATen/hip/HIPContext.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
