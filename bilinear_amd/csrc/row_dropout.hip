@@ -10,8 +10,8 @@
 // expectation of y is x.  The backward pass is the same map on dy: there is nothing to save.
 //
 // Bound by memory: 16384 x 2048 bf16 22.6 us = 5.9 TB/s of its bytes on three inputs in turn, 27 us = 5.0 where forward and
-// backward alternate on 800 MB (a copy of 537 MB: 5.0); a stored mask of one bit would add 6 % of the bytes each way.  16 bits
-// a draw make it 1/8 call an element: 32 bits, 1/4 call, would cost a 16-bit type more arithmetic than its bytes take.
+// backward alternate on 800 MB (a copy of 537 MB: 5.0); a stored mask of one bit would add 3 % to a 16-bit type's bytes
+// each way.  A draw takes 16 bits so that a call, 20 multiplies, serves 8 elements.
 #include "row_ops.h"
 #include "row_ops_dev.h"
 

@@ -20,6 +20,7 @@
 
 #include <optional>
 #include <tuple>
+#include <vector>
 
 #include "../../include/bilinear_hip.h"
 
@@ -250,7 +251,7 @@ variable_list residual_norm_backward_launch(const Tensor& dy, const Tensor& dh, 
 // A leaf's gradient accumulator belongs to the stream it was made on.  One that an eager graph on the DEFAULT stream still
 // holds cannot take part in a stream capture (that stream cannot be captured: the capture would break inside the autograd
 // engine, where the error ends the process), so such a call is refused before anything is enqueued.
-void refuse_eager_leaves(std::initializer_list<const Tensor*> inputs) {
+template <typename L> void refuse_eager_leaves(const L& inputs) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   for (const Tensor* t : inputs) {
     if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
@@ -353,7 +354,7 @@ Tensor layer_norm(const Tensor& x, const Optional& weight, const Optional& bias,
   check_eps(eps);
   const Tensor w = plain(weight), b = plain(bias);
   if (!wants_grad({&x, &w, &b})) return layer_norm_launch(x, dense(w), dense(b), eps, code, Moments());
-  refuse_eager_leaves({&x, &w, &b});
+  refuse_eager_leaves(std::initializer_list<const Tensor*>{&x, &w, &b});
   const Tensor both = both_moments(x);
   Tensor y = layer_norm_launch(x, dense(w), dense(b), eps, code, Moments(both));
   auto node = make_node<LayerNormBackward>();
@@ -372,7 +373,7 @@ Tensor dropout(const Tensor& x, double p, int64_t seed, int64_t step, int64_t la
   Draws d{p, seed, step, layer, row_offset, plain(device_step)};
   check_draws(d, x);
   const bool grad = wants_grad({&x});
-  if (grad) refuse_eager_leaves({&x});
+  if (grad) refuse_eager_leaves(std::initializer_list<const Tensor*>{&x});
   const Tensor used = grad ? used_step(d) : Tensor();
   Tensor y = dropout_launch(x, d, used);
   if (grad) {
@@ -398,7 +399,7 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& residual
   const Tensor w = plain(weight), b = plain(bias);
   const bool grad = wants_grad({&x, &residual, &w, &b});
   if (!grad) return residual_norm_launch(x, residual, dense(w), dense(b), eps, d, code, Moments(), Tensor());
-  refuse_eager_leaves({&x, &residual, &w, &b});
+  refuse_eager_leaves(std::initializer_list<const Tensor*>{&x, &residual, &w, &b});
   const Tensor both = both_moments(x);
   const Tensor used = used_step(d);
   auto [y, h] = residual_norm_launch(x, residual, dense(w), dense(b), eps, d, code, Moments(both), used);
@@ -512,6 +513,11 @@ PYBIND11_MODULE(_rows, m) {
   m.def("layer_norm", &layer_norm, release);
   m.def("dropout", &dropout, release);
   m.def("residual_norm", &residual_norm, release);
+  m.def("refuse_eager_leaves", [](const std::vector<Tensor>& tensors) {
+    std::vector<const Tensor*> at;
+    for (const Tensor& t : tensors) at.push_back(&t);
+    refuse_eager_leaves(at);
+  });
   m.def("op_layer_norm", &op_layer_norm, release);
   m.def("op_layer_norm_backward", &op_layer_norm_backward, release);
   m.def("op_row_dropout", &op_row_dropout, release);

@@ -115,7 +115,14 @@ def _pick(needed, grads):
     return tuple(g if n else None for n, g in zip(needed, grads))
 
 
+def _refuse_eager_leaves(inputs):
+    """In a stream capture: what the functions refuse (csrc/torch_rows.cpp), for calls of the operators themselves."""
+    if not torch.compiler.is_compiling() and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        _native().refuse_eager_leaves([t for t in inputs if isinstance(t, torch.Tensor)])
+
+
 def _ln_setup(ctx, inputs, output):
+    _refuse_eager_leaves(inputs)
     x, weight, bias, _ = inputs
     ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(x, weight, output[1], output[2])
@@ -129,6 +136,7 @@ def _ln_formula(ctx, dy, dmean, drstd):
 
 
 def _drop_setup(ctx, inputs, output):
+    _refuse_eager_leaves(inputs)
     _, p, seed, step, layer, row_offset, device_step = inputs
     ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(*(() if device_step is None else (output[1],)))
@@ -141,6 +149,7 @@ def _drop_formula(ctx, dy, dused):
 
 
 def _res_setup(ctx, inputs, output):
+    _refuse_eager_leaves(inputs)
     x, residual, weight, bias, _, p, seed, step, layer, row_offset, device_step = inputs
     ctx.mark_non_differentiable(*output[2:])
     ctx.save_for_backward(output[1], weight, output[2], output[3], None if device_step is None else output[4])

@@ -511,10 +511,39 @@ def test_capture_with_a_live_eager_graph_is_refused(B):
     with torch.cuda.graph(graph):
         with pytest.raises(RuntimeError, match="still part of an eager autograd graph"):
             B.layer_norm(x, w, b)
-        x.add_(1)                # (something for the graph to hold)
+        with pytest.raises(RuntimeError, match="still part of an eager autograd graph"):
+            torch.ops.bilinear_hip.layer_norm(x, w, b, 1e-5)
+        with torch.no_grad():
+            z = B.layer_norm(x, w, b)      # nothing to differentiate: nothing to refuse
     graph.replay()
     torch.cuda.synchronize()
-    assert torch.isfinite(eager).all()
+    assert torch.equal(z, eager)
+
+
+def test_a_captured_backward_beside_a_live_graph_of_a_side_stream(B):
+    """The usual warm-up: eager steps on a side stream whose outputs are still held when the capture begins."""
+    x, dy = data(64, 128, F32, 1).requires_grad_(), data(64, 128, F32, 2)
+    w, b = params(128, F32, 5)
+    torch.autograd.graph.set_warn_on_accumulate_grad_stream_mismatch(False)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        held = B.layer_norm(x, w, b)
+        held.backward(dy)
+    torch.cuda.current_stream().wait_stream(side)
+    want = [t.grad.clone() for t in (x, w, b)]
+    x.grad = w.grad = b.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        B.layer_norm(x, w, b).backward(dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for t, v in zip((x, w, b), want):
+            assert torch.equal(t.grad, v)
+            t.grad.zero_()
+    assert torch.isfinite(held).all()
+    torch.autograd.graph.set_warn_on_accumulate_grad_stream_mismatch(True)
 
 
 def test_under_torch_compile(B):
