@@ -222,9 +222,11 @@ class _Draws:
     gets its own, as every stand-alone stage does) and, as the step, a number from torch's CPU generator — so
     ``torch.manual_seed`` repeats the masks, a saved generator state continues them and a checkpointed block (which
     restores that state) is recomputed with the mask it had.  In a captured graph such a number would be frozen: give the
-    module an int64 device tensor (``set_device_step``) that the graph advances between replays."""
+    module an int64 device tensor (``set_device_step``) that the graph advances between replays.  ``row_offset``: the
+    global index of this process's first row, so that ranks with one seed draw the parts of one mask."""
 
     _device_step = None
+    row_offset = 0
 
     def _init_draws(self):
         from .model.bilinear import _HeavyLinear
@@ -252,8 +254,11 @@ class _Draws:
                                    "(set_device_step): every replay would draw the same mask")
             # calls of one captured step differ in the upper half of the step, replays in the device's count
             self._captured += 1
-            return {"seed": self._seed, "step": self._captured << 32, "layer": self._layer, "device_step": self._device_step}
-        return {"seed": self._seed, "step": int(torch.empty((), dtype=torch.int64).random_()), "layer": self._layer}
+            step, device_step = self._captured << 32, self._device_step
+        else:
+            step, device_step = int(torch.empty((), dtype=torch.int64).random_()), None
+        return {"seed": self._seed, "step": step, "layer": self._layer, "row_offset": self.row_offset,
+                "device_step": device_step}
 
 
 class Dropout(_Draws, nn.Dropout):

@@ -320,6 +320,19 @@ def test_mask_does_not_depend_on_how_rows_are_spread(B):
     assert torch.equal(B.dropout(wide, 0.4, seed=3, step=2) != 0, whole != 0)
 
 
+def test_modules_of_two_ranks_draw_the_parts_of_one_mask(B):
+    x = data(96, 50, F32, 1)
+    drop, norm = B.Dropout(0.4), B.ResidualNorm(50, p=0.4).cuda()
+
+    def call(rows, offset):
+        torch.manual_seed(5)                       # what every rank does
+        drop.row_offset = norm.row_offset = offset
+        return drop(x[rows]), norm(x[rows], x[rows])[1]
+    whole, lower, upper = call(slice(None), 0), call(slice(0, 40), 0), call(slice(40, 96), 40)
+    for w, a, b in zip(whole, lower, upper):
+        assert torch.equal(torch.cat((a, b)), w)
+
+
 # ---- residual norm --------------------------------------------------------------------------------------------------
 
 def check_residual_norm(B, x, r, w, b, dy, dh, p, eps=1e-5):
@@ -654,7 +667,11 @@ def test_a_residual_network_of_the_operators_trains(B):
     state = torch.get_rng_state()
     torch.nn.functional.mse_loss(net(x), t).backward()
     torch.set_rng_state(state)                # the numbers the modules drew, in the order of their calls
-    masks = [R.factor(rows, width, p, **m._next_draws()) for m in [net.drop, *net.norms]]
+    masks = []
+    for m in [net.drop, *net.norms]:
+        kw = m._next_draws()
+        assert kw.pop("device_step") is None
+        masks.append(R.factor(rows, width, p, **kw))
 
     P = {k: v.detach().double().cpu().requires_grad_() for k, v in net.named_parameters()}
     h = (d(x) @ P["encode.weight"].t() + P["encode.bias"]) * masks[0]
