@@ -522,8 +522,13 @@ template <typename T, typename R, bool RESID, int LANES, int NV, bool SHORT = fa
 static int launch_fwd_rows(hipStream_t s, const NormFwd& p) {
   constexpr int BLOCK = LANES > 256 ? LANES : 256;
   // at most 8 blocks of 256 threads a CU, which walk the rows with the parameters in registers: 16384 x 2048 bf16 layer
-  // norm 22.4 us, one group of rows a block (parameters read for each) 27.6
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), 2048 * 256 / BLOCK);
+  // norm 22.4 us, one group of rows a block (parameters read for each) 27.6.  The layer norm of rows of 1 to 4 KiB runs
+  // better in 6 a CU (4096 x 1024 fp32 8.4 against 9.5 us, 16384 x 1001 fp16 12.2 against 13.3, 16384 x 1024 bf16 11.6
+  // against 12.0); shorter rows (65536 x 256 bf16 13.7 against 12.8) and the residual norm (16384 x 2048 bf16 47.0 against
+  // 44.3) do not.
+  constexpr int bytes = LANES * NV * ROW_UNIT * (int)sizeof(T);
+  constexpr int most = (!RESID && NV <= 2 && bytes >= 1024 && bytes <= 4096 ? 6 : 8) * 256;
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(p.rows, BLOCK / LANES), most * 256 / BLOCK);
   hipLaunchKernelGGL((norm_fwd_rows_kernel<T, R, RESID, LANES, NV, BLOCK, SHORT>), dim3(blocks), dim3(BLOCK), 0, s, p);
   BLH_HIP_TRY(hipGetLastError());
   return BLH_OK;

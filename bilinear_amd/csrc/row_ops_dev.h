@@ -108,8 +108,8 @@ template <> struct RawUnit<float> {
 //             last 8 elements instead, which lie inside the row (SHORT: rows of fewer than 8 elements, element by element to
 //             the same places);
 //   settle    moves such a unit down and leaves zeros behind the row's end; `width` 0 makes it all zeros.
-// (16384 x 1001 fp16: layer norm 13.2 us, backward 24.7; with the shift inside the load 18.9 and 29.9, with a branch around
-// element loads 14.7 and 27.0; 16384 x 1000 takes 12.7 and 23.4.)
+// (16384 x 1001 fp16: layer norm 12.2 us, backward 24.7; with the shift inside the load 18.9 and 29.9, with a branch around
+// element loads 14.7 and 27.0; 16384 x 1000 takes 12.0 and 23.4.)
 template <bool SHORT, typename T> __device__ __forceinline__ RawUnit<T> load_raw(const T* row, int c, int width) {
   RawUnit<T> r;
   if constexpr (!SHORT) {
