@@ -111,16 +111,17 @@ __global__ __launch_bounds__(256) void norm_bwd_rows_kernel(NormBwd p) {
     const float mean = p.mean[row], rstd = p.rstd[row];
     float s1 = 0.f, s2 = 0.f;
     for (int u = threadIdx.x; u < units; u += 256) {
-      float d[ROW_UNIT], f[ROW_UNIT], g[ROW_UNIT];
+      float g[ROW_UNIT];
       const int c = u * ROW_UNIT;
-      load_unit<false>(dy, c, W, d);
-      load_unit<false>(h, c, W, f);
+      RawUnit<T> d = load_raw<false>(dy, c, W);
+      RawUnit<R> f = load_raw<false>(h, c, W);
+      settle2(d, f, c, W);
       load_param_unit<false, T>(p.gamma, p.same, c, W, 1.f, g);
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e) {
-        const float t = d[e] * g[e];          // (zero behind the row's end: dy is)
+        const float t = d.get(e) * g[e];          // (zero behind the row's end: dy is)
         s1 += t;
-        s2 = fmaf(t, (f[e] - mean) * rstd, s2);
+        s2 = fmaf(t, (f.get(e) - mean) * rstd, s2);
       }
     }
     const float c1 = block_sum(s1, sh) / (float)W;
@@ -428,8 +429,7 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(NormBwd p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * ROW_UNIT;
-      settle(in.d[i], c, width);                   // (dy is 0 behind the row's end)
-      settle(in.f[i], c, width);
+      settle2(in.d[i], in.f[i], c, width);         // (dy is 0 behind the row's end and in a group without a row)
 #pragma unroll
       for (int e = 0; e < ROW_UNIT; ++e) {
         const float v = in.d[i].get(e), hat = (in.f[i].get(e) - in.mean) * in.rstd, t = v * gm[i][e];

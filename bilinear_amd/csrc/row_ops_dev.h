@@ -35,6 +35,13 @@ template <typename T> struct RawUnit {
     hi = s < 64 ? hi >> s : 0;
     q = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
   }
+  // the same, the dropped elements enter behind
+  __device__ __forceinline__ void rotate(int k) {
+    if (k & 4) q = u32x4{q[2], q[3], q[0], q[1]};
+    if (k & 2) q = u32x4{q[1], q[2], q[3], q[0]};
+    if (k & 1)
+      q = u32x4{q[0] >> 16 | q[1] << 16, q[1] >> 16 | q[2] << 16, q[2] >> 16 | q[3] << 16, q[3] >> 16 | q[0] << 16};
+  }
   // the first n elements (1 .. 7)
   __device__ __forceinline__ void store_some(T* p, int n) const {
     typedef uint64_t w4 __attribute__((aligned(2)));
@@ -80,6 +87,14 @@ template <> struct RawUnit<float> {
     if (k & 2) { q[0] = f32x4{q[0][2], q[0][3], q[1][0], q[1][1]}; q[1] = f32x4{q[1][2], q[1][3], 0.f, 0.f}; }
     if (k & 1) { q[0] = f32x4{q[0][1], q[0][2], q[0][3], q[1][0]}; q[1] = f32x4{q[1][1], q[1][2], q[1][3], 0.f}; }
   }
+  __device__ __forceinline__ void rotate(int k) {
+    const f32x4 a = q[0], b = q[1];
+    if (k & 4) { q[0] = b; q[1] = a; }
+    const f32x4 c = q[0], d = q[1];
+    if (k & 2) { q[0] = f32x4{c[2], c[3], d[0], d[1]}; q[1] = f32x4{d[2], d[3], c[0], c[1]}; }
+    const f32x4 u = q[0], v = q[1];
+    if (k & 1) { q[0] = f32x4{u[1], u[2], u[3], v[0]}; q[1] = f32x4{v[1], v[2], v[3], u[0]}; }
+  }
   __device__ __forceinline__ void store_some(float* p, int n) const {
     typedef float pair __attribute__((ext_vector_type(2)));
     typedef pair pair4 __attribute__((aligned(4)));
@@ -107,7 +122,10 @@ template <> struct RawUnit<float> {
 //   load_raw  reads 16 (32) bytes without a branch — a unit that crosses the row's end, or lies behind it, reads the row's
 //             last 8 elements instead, which lie inside the row (SHORT: rows of fewer than 8 elements, element by element to
 //             the same places);
-//   settle    moves such a unit down and leaves zeros behind the row's end; `width` 0 makes it all zeros.
+//   settle    moves such a unit down and leaves zeros behind the row's end; `width` 0 makes it all zeros;
+//   settle2   settles a gradient and, beside it, what is normalised, with elements of the same row (of the last one, in a group
+//             without a row) behind the row's end: (0 - mean) rstd may pass the largest number, whose product with the gradient's
+//             0 is NaN, where a row's own elements make NaN only if the row's results are.
 // (16384 x 1001 fp16: layer norm 12.2 us, backward 24.7; with the shift inside the load 18.9 and 29.9, with a branch around
 // element loads 14.7 and 27.0; 16384 x 1000 takes 12.0 and 23.4.)
 template <bool SHORT, typename T> __device__ __forceinline__ RawUnit<T> load_raw(const T* row, int c, int width) {
@@ -117,7 +135,7 @@ template <bool SHORT, typename T> __device__ __forceinline__ RawUnit<T> load_raw
   } else {
     float f[ROW_UNIT];
 #pragma unroll
-    for (int e = 0; e < ROW_UNIT; ++e) f[e] = e >= ROW_UNIT - width ? (float)row[e - (ROW_UNIT - width)] : 0.f;
+    for (int e = 0; e < ROW_UNIT; ++e) f[e] = (float)row[max(0, e - (ROW_UNIT - width))];
     r.set(f);
   }
   return r;
@@ -126,6 +144,16 @@ template <typename T> __device__ __forceinline__ void settle(RawUnit<T>& r, int 
   if (c + ROW_UNIT > width) {
     if (c < width) r.shift(c + ROW_UNIT - width);
     else r.zero();
+  }
+}
+template <typename T, typename R> __device__ __forceinline__ void settle2(RawUnit<T>& d, RawUnit<R>& f, int c, int width) {
+  if (c + ROW_UNIT > width) {
+    if (c < width) {
+      d.shift(c + ROW_UNIT - width);
+      f.rotate(c + ROW_UNIT - width);
+    } else {
+      d.zero();
+    }
   }
 }
 
