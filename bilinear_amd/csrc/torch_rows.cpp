@@ -265,9 +265,15 @@ template <typename L> void refuse_eager_leaves(const L& inputs) {
   }
 }
 
-// The formulas below are not themselves differentiable: a backward pass through them is refused where it is asked for.
+// The norms' formulas below are not themselves differentiable: under create_graph their results refuse a backward pass through
+// them.  (The error's node is attached to tensors that need a gradient alone, which fresh results do not.)
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    g.set_requires_grad(true);
+  }
   const auto error = std::make_shared<torch::autograd::DelayedError>(
       "bilinear_amd row operators: trying to differentiate the backward pass, which is not supported", (int64_t)grads.size());
   return (*error)(std::move(grads));
@@ -293,12 +299,18 @@ struct LayerNormBackward : public torch::autograd::Node {
   }
 };
 
+Tensor dropout(const Tensor& x, double p, int64_t seed, int64_t step, int64_t layer, int64_t row_offset,
+               const Optional& device_step);
+
+// dropout is linear: its backward is the same map, with the same derivative
 struct RowDropoutBackward : public torch::autograd::Node {
   Draws d;
   std::string name() const override { return "BilinearRowDropoutBackward"; }
   variable_list apply(variable_list&& grads) override {
     if (!grads[0].defined()) return variable_list(1);
-    return once({dropout_launch(grads[0], d, Tensor())});
+    if (!at::GradMode::is_enabled()) return {dropout_launch(grads[0], d, Tensor())};
+    return {dropout(grads[0], d.p, d.seed, d.step, d.layer, d.row_offset,
+                    d.device_step.defined() ? Optional(d.device_step) : Optional())};
   }
 };
 

@@ -11,6 +11,8 @@ batch and no stored mask.  Three surfaces, as for the lifter:
     bilinear_amd.LayerNorm(1024), .Dropout(0.1), .ResidualNorm(1024, p=0.1)     # modules
     torch.ops.bilinear_hip.{layer_norm, row_dropout, residual_norm, ...}        # custom operators (torch.compile)
 
+Second derivatives: those of dropout; a backward pass through the norms' gradients is refused.
+
 The last axis is the row.  Types: x float32 / bfloat16 / float16; weight and bias float32 or x's type; the residual
 stream (``residual``, ``h``) float32 or x's type.  Rows of a wider tensor (last axis dense) are read in place.  Tensors
 must live on a HIP device: there is no CPU path.
@@ -164,9 +166,15 @@ def _res_formula(ctx, dy, dh, *unused):
         dy, dh, h, weight, mean, rstd, *ctx.draws, used, *need, ctx.code)) + (None,) * 7
 
 
+def _not_twice(ctx, *grads):
+    raise RuntimeError("bilinear_amd row operators: trying to differentiate the backward pass, which is not supported")
+
+
 torch.library.register_autograd("bilinear_hip::layer_norm", _ln_formula, setup_context=_ln_setup, lib=_LIB)
 torch.library.register_autograd("bilinear_hip::row_dropout", _drop_formula, setup_context=_drop_setup, lib=_LIB)
 torch.library.register_autograd("bilinear_hip::residual_norm", _res_formula, setup_context=_res_setup, lib=_LIB)
+torch.library.register_autograd("bilinear_hip::layer_norm_backward", _not_twice, lib=_LIB)
+torch.library.register_autograd("bilinear_hip::residual_norm_backward", _not_twice, lib=_LIB)
 
 
 # ---- functions ------------------------------------------------------------------------------------------------------

@@ -14,6 +14,65 @@ def B():
     return bilinear_amd
 
 
+# ---- second derivatives ---------------------------------------------------------------------------------------------
+
+def _first_outputs(B):
+    op = torch.ops.bilinear_hip
+    return {
+        "layer_norm": lambda x, r, w, b: B.layer_norm(x, w, b),
+        "residual_norm": lambda x, r, w, b: B.residual_norm(x, r, w, b, p=0.3, seed=1)[0],
+        "residual_norm's stream": lambda x, r, w, b: B.residual_norm(x, r, w, b, p=0.3, seed=1)[1],
+        "residual_norm without dropout": lambda x, r, w, b: B.residual_norm(x, r, w, b)[0],
+        "operator layer_norm": lambda x, r, w, b: op.layer_norm(x, w, b, 1e-5)[0],
+        "operator residual_norm": lambda x, r, w, b: op.residual_norm(x, r, w, b, 1e-5, 0.3, 1, 0, 0, 0, None)[0],
+    }
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "residual_norm", "residual_norm's stream", "residual_norm without dropout",
+                                  "operator layer_norm", "operator residual_norm"])
+def test_a_second_derivative_is_refused_beside_other_terms(B, name):
+    """A gradient penalty in a loss that has other gradients: its share must not be dropped in silence."""
+    x, r = data(3, 16, F32, 1).requires_grad_(), data(3, 16, F32, 2).requires_grad_()
+    w, b = params(16, F32, 5)
+    y = _first_outputs(B)[name](x, r, w, b)
+    g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    assert g.requires_grad
+    with pytest.raises(RuntimeError, match="differentiate the backward pass"):
+        (y.sum() + g.square().sum()).backward()
+
+
+def test_the_backward_operators_refuse_to_be_differentiated(B):
+    op = torch.ops.bilinear_hip
+    x, dy = data(3, 16, F32, 1), data(3, 16, F32, 2).requires_grad_()
+    w = params(16, F32, 5)[0]
+    with torch.no_grad():
+        _, mean, rstd = op.layer_norm(x, w, None, 1e-5)
+    dx = op.layer_norm_backward(dy, x, w, mean, rstd, True, True, True, 0)[0]
+    with pytest.raises(RuntimeError, match="differentiate the backward pass"):
+        (dx.sum() + dy.sum()).backward()
+    dx = op.residual_norm_backward(dy, None, x, w, mean, rstd, 0.3, 1, 0, 0, 0, None, True, True, True, True, 0)[0]
+    with pytest.raises(RuntimeError, match="differentiate the backward pass"):
+        (dx.sum() + dy.sum()).backward()
+
+
+@pytest.mark.parametrize("operator", [False, True])
+@pytest.mark.parametrize("device_step", [False, True])
+def test_second_derivative_of_dropout(B, operator, device_step):
+    """f: the factor of an element.  y = f x, g = d(sum y^3)/dx = 3 f^3 x^2, d(sum g^2 + sum y)/dx = 36 f^6 x^3 + f: some
+    fifteen fp32 products, of half a step each."""
+    x = data(20, 40, F32, 1).requires_grad_()
+    step = torch.full((1,), 4, dtype=torch.int64, device="cuda") if device_step else None
+    args = (0.3, 7, 1 if device_step else 5, 2, 3, step)
+    y = torch.ops.bilinear_hip.row_dropout(x, *args)[0] if operator else B.dropout(x, *args)
+    if device_step:
+        step.add_(1)                     # the backward passes read the step that the forward used
+    g, = torch.autograd.grad(y.pow(3).sum(), x, create_graph=True)
+    got, = torch.autograd.grad(g.square().sum() + y.sum(), x)
+    f = R.factor(20, 40, 0.3, seed=7, step=5, layer=2, row_offset=3)
+    want = 36 * f ** 6 * d(x) ** 3 + f
+    R.close(got, want, 24 * R.U * (36 * f ** 6 * d(x).abs() ** 3 + f) + R.tiny(F32), "second derivative")
+
+
 # ---- values at the ends of the range ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,width", [(2, 12), (3, 64), (1025, 64), (1026, 12), (1027, 5), (1027, 200), (2, 20004)])
