@@ -5,10 +5,13 @@
 // and autograd runs a backward node on its device thread, where a Python node starts with cold caches.  Measured with
 // ctypes and a Python autograd.Function: forward + backward of a 64 x 1024 layer norm 143 us, without a gradient 12.6; with
 // these nodes 40-64 us (23.6 with single-threaded autograd; the kernels are 8) and 4.3-5.
+#include <ATen/TracerMode.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
@@ -246,6 +249,70 @@ variable_list residual_norm_backward_launch(const Tensor& dy, const Tensor& dh, 
   return {dx, dres, g.weight, g.bias};
 }
 
+// ---- through the dispatcher -------------------------------------------------------------------------------------------
+// A tracer, a dispatch mode or a tensor subclass sees what goes through torch's dispatcher.  The calls below do not — it would
+// see an allocation and nothing that fills it — so that where one is present the custom operators (row_ops.py) take their
+// place: outputs that were not asked for come back empty there, and autograd is the operators' own.
+
+bool followed(std::initializer_list<const Tensor*> inputs) {
+  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::dispatch_mode_enabled()) return true;
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->key_set().has(c10::DispatchKey::Python)) return true;
+  return false;
+}
+
+template <typename Signature> c10::TypedOperatorHandle<Signature> custom(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+
+Optional given(const Tensor& t) { return t.defined() ? Optional(t) : Optional(); }
+Tensor wanted(bool need, const Tensor& t) { return need ? t : Tensor(); }
+
+std::tuple<Tensor, Tensor, Tensor> custom_layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Optional&, const Optional&, double)>(
+      "bilinear_hip::layer_norm");
+  return op.call(x, given(w), given(b), eps);
+}
+
+variable_list custom_layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& moments,
+                                         bool need_x, bool need_weight, bool need_bias, int64_t code) {
+  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor>(
+      const Tensor&, const Tensor&, const Optional&, const Tensor&, const Tensor&, bool, bool, bool, int64_t)>(
+      "bilinear_hip::layer_norm_backward");
+  const auto [dx, dw, db] = op.call(dy, x, given(w), moments.select(0, 0), moments.select(0, 1), need_x, need_weight,
+                                    need_bias, code);
+  return {wanted(need_x, dx), wanted(need_weight, dw), wanted(need_bias, db)};
+}
+
+Tensor custom_dropout(const Tensor& x, const Draws& d) {
+  static const auto op = custom<std::tuple<Tensor, Tensor>(const Tensor&, double, c10::SymInt, c10::SymInt, c10::SymInt,
+                                                           c10::SymInt, const Optional&)>("bilinear_hip::row_dropout");
+  return std::get<0>(op.call(x, d.p, d.seed, d.step, d.layer, d.row_offset, given(d.device_step)));
+}
+
+std::tuple<Tensor, Tensor> custom_residual_norm(const Tensor& x, const Tensor& residual, const Tensor& w, const Tensor& b,
+                                                double eps, const Draws& d) {
+  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>(
+      const Tensor&, const Tensor&, const Optional&, const Optional&, double, double, c10::SymInt, c10::SymInt, c10::SymInt,
+      c10::SymInt, const Optional&)>("bilinear_hip::residual_norm");
+  const auto out = op.call(x, residual, given(w), given(b), eps, d.p, d.seed, d.step, d.layer, d.row_offset,
+                           given(d.device_step));
+  return {std::get<0>(out), std::get<1>(out)};
+}
+
+variable_list custom_residual_norm_backward(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w,
+                                            const Tensor& moments, const Draws& d, bool need_x, bool need_residual,
+                                            bool need_weight, bool need_bias, int64_t code) {
+  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+      const Tensor&, const Optional&, const Tensor&, const Optional&, const Tensor&, const Tensor&, double, c10::SymInt,
+      c10::SymInt, c10::SymInt, c10::SymInt, const Optional&, bool, bool, bool, bool, int64_t)>(
+      "bilinear_hip::residual_norm_backward");
+  const auto [dx, dres, dw, db] = op.call(dy, given(dh), h, given(w), moments.select(0, 0), moments.select(0, 1), d.p, d.seed,
+                                          d.step, d.layer, d.row_offset, given(d.device_step), need_x, need_residual,
+                                          need_weight, need_bias, code);
+  return {wanted(need_x, dx), wanted(need_residual, dres), wanted(need_weight, dw), wanted(need_bias, db)};
+}
+
 // ---- autograd -------------------------------------------------------------------------------------------------------
 
 // A leaf's gradient accumulator belongs to the stream it was made on.  One that an eager graph on the DEFAULT stream still
@@ -293,9 +360,12 @@ struct LayerNormBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(3);
-    const Tensor in = x.unpack(), w = dense(weight.unpack());
-    return once(layer_norm_backward_launch(grads[0], in, w, Moments(moments), task_should_compute_output(0),
-                                           task_should_compute_output(1), task_should_compute_output(2), code));
+    const Tensor in = x.unpack(), w = weight.unpack();
+    const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1),
+               need_b = task_should_compute_output(2);
+    if (followed({&grads[0], &in, &w}))
+      return custom_layer_norm_backward(grads[0], in, w, moments, need_x, need_w, need_b, code);
+    return once(layer_norm_backward_launch(grads[0], in, dense(w), Moments(moments), need_x, need_w, need_b, code));
   }
 };
 
@@ -308,9 +378,8 @@ struct RowDropoutBackward : public torch::autograd::Node {
   std::string name() const override { return "BilinearRowDropoutBackward"; }
   variable_list apply(variable_list&& grads) override {
     if (!grads[0].defined()) return variable_list(1);
-    if (!at::GradMode::is_enabled()) return {dropout_launch(grads[0], d, Tensor())};
-    return {dropout(grads[0], d.p, d.seed, d.step, d.layer, d.row_offset,
-                    d.device_step.defined() ? Optional(d.device_step) : Optional())};
+    if (!at::GradMode::is_enabled() && !followed({&grads[0]})) return {dropout_launch(grads[0], d, Tensor())};
+    return {dropout(grads[0], d.p, d.seed, d.step, d.layer, d.row_offset, given(d.device_step))};
   }
 };
 
@@ -330,15 +399,17 @@ struct ResidualNormBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(4);
-    const Tensor stream = h.unpack(shared_from_this()), w = dense(weight.unpack());
+    const Tensor stream = h.unpack(shared_from_this()), w = weight.unpack();
     // only the stream went on: the norm's share is zero
     const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(stream.sizes(), stream.options().dtype(dtype));
-    const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1);
+    const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1),
+               need_w = task_should_compute_output(2), need_b = task_should_compute_output(3);
+    if (followed({&dy, &grads[1], &stream, &w}))
+      return custom_residual_norm_backward(dy, grads[1], stream, w, moments, d, need_x, need_r, need_w, need_b, code);
     // without dropout and with one type both branches of the sum get the same gradient: it is written once
     const bool same = need_x && need_r && stream.scalar_type() == dtype && (int64_t)(d.p * 65536.0 + 0.5) == 0;
-    variable_list out = residual_norm_backward_launch(dy, grads[1], stream, w, Moments(moments), d, need_x && !same,
-                                                      need_r, task_should_compute_output(2),
-                                                      task_should_compute_output(3), code);
+    variable_list out = residual_norm_backward_launch(dy, grads[1], stream, dense(w), Moments(moments), d, need_x && !same,
+                                                      need_r, need_w, need_b, code);
     if (same) out[0] = out[1];
     return once(std::move(out));
   }
@@ -365,6 +436,7 @@ Tensor layer_norm(const Tensor& x, const Optional& weight, const Optional& bias,
   const int32_t code = check_params(x, weight, bias);
   check_eps(eps);
   const Tensor w = plain(weight), b = plain(bias);
+  if (followed({&x, &w, &b})) return std::get<0>(custom_layer_norm(x, w, b, eps));
   if (!wants_grad({&x, &w, &b})) return layer_norm_launch(x, dense(w), dense(b), eps, code, Moments());
   refuse_eager_leaves(std::initializer_list<const Tensor*>{&x, &w, &b});
   const Tensor both = both_moments(x);
@@ -384,6 +456,7 @@ Tensor dropout(const Tensor& x, double p, int64_t seed, int64_t step, int64_t la
   check_rows(x, "x");
   Draws d{p, seed, step, layer, row_offset, plain(device_step)};
   check_draws(d, x);
+  if (followed({&x, &d.device_step})) return custom_dropout(x, d);
   const bool grad = wants_grad({&x});
   if (grad) refuse_eager_leaves(std::initializer_list<const Tensor*>{&x});
   const Tensor used = grad ? used_step(d) : Tensor();
@@ -409,6 +482,7 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& residual
   Draws d{p, seed, step, layer, row_offset, plain(device_step)};
   check_draws(d, x);
   const Tensor w = plain(weight), b = plain(bias);
+  if (followed({&x, &residual, &w, &b, &d.device_step})) return custom_residual_norm(x, residual, w, b, eps, d);
   const bool grad = wants_grad({&x, &residual, &w, &b});
   if (!grad) return residual_norm_launch(x, residual, dense(w), dense(b), eps, d, code, Moments(), Tensor());
   refuse_eager_leaves(std::initializer_list<const Tensor*>{&x, &residual, &w, &b});

@@ -9,7 +9,10 @@ batch and no stored mask.  Three surfaces, as for the lifter:
     y = bilinear_amd.dropout(x, 0.1, seed=7, step=3, layer=0)
     y, h = bilinear_amd.residual_norm(x, h, weight, bias, p=0.1, seed=7, step=3, layer=1)
     bilinear_amd.LayerNorm(1024), .Dropout(0.1), .ResidualNorm(1024, p=0.1)     # modules
-    torch.ops.bilinear_hip.{layer_norm, row_dropout, residual_norm, ...}        # custom operators (torch.compile)
+    torch.ops.bilinear_hip.{layer_norm, row_dropout, residual_norm, ...}        # custom operators (torch.compile, tracers)
+
+The functions go to the library directly.  Under a tracer (torch.jit.trace, make_fx), a dispatch mode, or with tensor
+subclasses, they call the custom operators, which these can see.
 
 Second derivatives: those of dropout; a backward pass through the norms' gradients is refused.
 
@@ -256,6 +259,9 @@ class _Draws:
     def _next_draws(self):
         if self._seed is None:
             self._seed = int(torch.initial_seed()) & ((1 << 63) - 1)
+        if torch.jit.is_tracing():
+            raise RuntimeError("bilinear_amd: dropout in a trace: every call would draw the same mask.  Trace the module in "
+                               "eval mode, or the function `dropout` with a device_step")
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             if self._device_step is None:
                 raise RuntimeError("bilinear_amd: dropout in a stream capture needs a step on the device "

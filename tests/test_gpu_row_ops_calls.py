@@ -73,6 +73,105 @@ def test_second_derivative_of_dropout(B, operator, device_step):
     R.close(got, want, 24 * R.U * (36 * f ** 6 * d(x).abs() ** 3 + f) + R.tiny(F32), "second derivative")
 
 
+# ---- tracers --------------------------------------------------------------------------------------------------------
+
+def _functions(B):
+    def norm(x, r, w, b):
+        return B.layer_norm(x, w, b)
+
+    def drop(x, r, w, b):
+        return B.dropout(x, 0.3, 5, 7, 1)
+
+    def residual(x, r, w, b):
+        return B.residual_norm(x, r, w, b, 1e-5, 0.3, 5, 7, 1)
+    return {"layer_norm": norm, "dropout": drop, "residual_norm": residual}
+
+
+def _inputs(seed, grad=False):
+    return tuple(t.requires_grad_(grad) for t in (data(6, 40, BF16, seed), data(6, 40, F32, seed + 1),
+                                                   data(1, 40, F32, seed + 2)[0], data(1, 40, F32, seed + 3)[0]))
+
+
+def _equal(got, want):
+    got, want = (t if isinstance(t, (tuple, list)) else (t,) for t in (got, want))
+    assert len(got) == len(want)
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "dropout", "residual_norm"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_jit_trace_holds_the_operator(B, name, grad):
+    f = _functions(B)[name]
+    traced = torch.jit.trace(f, _inputs(1, grad))
+    assert "bilinear_hip::" in str(traced.graph)
+    for seed in (1, 10):
+        args = _inputs(seed, grad)
+        got, want = traced(*args), f(*args)
+        _equal(got, want)
+        if grad:
+            (got, want) = ((t,) if torch.is_tensor(t) else t for t in (got, want))
+            ones = [torch.ones_like(t) for t in want]
+            wrt = args[:1] if name == "dropout" else args if name == "residual_norm" else (args[0], *args[2:])
+            _equal(torch.autograd.grad(got, wrt, ones), torch.autograd.grad(want, wrt, ones))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "dropout", "residual_norm"])
+def test_make_fx_holds_the_operator_and_its_backward(B, name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f = _functions(B)[name]
+    _equal(make_fx(f)(*_inputs(1))(*_inputs(10)), f(*_inputs(10)))
+
+    def step(x, r, w, b):
+        x = x.detach().requires_grad_()
+        out = f(x, r, w, b)
+        out = out if torch.is_tensor(out) else out[0]
+        return torch.autograd.grad(out, x, torch.ones_like(out))[0]
+    graph = make_fx(step)(*_inputs(1))
+    assert sum(str(n.target).startswith("bilinear_hip.") for n in graph.graph.nodes) == 2
+    _equal(graph(*_inputs(10)), step(*_inputs(10)))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "dropout", "residual_norm"])
+def test_the_backward_of_an_eager_graph_under_make_fx(B, name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    args = _inputs(1, True)
+    out = _functions(B)[name](*args)
+    out = (out,) if torch.is_tensor(out) else out
+    wrt = args[:1] if name == "dropout" else args if name == "residual_norm" else (args[0], *args[2:])
+    back = lambda *dy: torch.autograd.grad(out, wrt, dy, retain_graph=True)    # noqa: E731
+    one, two = ([data(6, 40, t.dtype, s + k) for k, t in enumerate(out)] for s in (20, 30))
+    graph = make_fx(back)(*one)
+    assert any(str(n.target).startswith("bilinear_hip.") for n in graph.graph.nodes)
+    _equal(graph(*two), back(*two))
+
+
+def test_a_dispatch_mode_sees_the_operators(B):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            names.append(str(func))
+            return func(*args, **(kwargs or {}))
+    names, args = [], _inputs(1, True)
+    want = [f(*args) for f in _functions(B).values()]
+    with Seen():
+        got = [f(*args) for f in _functions(B).values()]
+    for p, q in zip(got, want):
+        _equal(p, q)
+    assert [n for n in names if n.startswith("bilinear_hip.")] == [
+        "bilinear_hip.layer_norm.default", "bilinear_hip.row_dropout.default", "bilinear_hip.residual_norm.default"]
+
+
+def test_modules_that_drop_are_not_traced_with_one_mask(B):
+    x = data(6, 40, F32, 1)
+    for m, args in ((B.Dropout(0.3), (x,)), (B.ResidualNorm(40, p=0.3).cuda(), (x, x))):
+        with pytest.raises(RuntimeError, match="every call would draw the same mask"):
+            torch.jit.trace(m, args)
+        traced = torch.jit.trace(m.eval(), args)
+        _equal(traced(*args), m(*args))
+
+
 # ---- values at the ends of the range ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,width", [(2, 12), (3, 64), (1025, 64), (1026, 12), (1027, 5), (1027, 200), (2, 20004)])

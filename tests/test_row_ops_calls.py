@@ -1,0 +1,44 @@
+"""Row operators without a GPU under the calls around them: tracers and shape propagation."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+
+import bilinear_amd as B
+
+
+def _shapes(*tensors):
+    return [(tuple(t.shape), t.dtype, t.device.type) for t in tensors]
+
+
+def test_functions_propagate_shapes_under_a_fake_mode():
+    with FakeTensorMode():
+        x, r = torch.empty(3, 5, 48, dtype=torch.bfloat16, device="cuda"), torch.empty(3, 5, 48, device="cuda")
+        w = torch.empty(48, device="cuda")
+        step = torch.zeros(1, dtype=torch.int64, device="cuda")
+        assert _shapes(B.layer_norm(x, w, w)) == _shapes(x)
+        assert _shapes(B.dropout(x, 0.3, seed=1, device_step=step)) == _shapes(x)
+        assert _shapes(*B.residual_norm(x, r, w, None, p=0.3, seed=1)) == _shapes(x, r)
+        with pytest.raises(RuntimeError, match="weight has shape"):         # the checks come first
+            B.layer_norm(x, torch.empty(47, device="cuda"))
+    assert _shapes(B.layer_norm(x, w, w)) == _shapes(x)                     # fake tensors outside their mode
+
+
+@pytest.mark.parametrize("name,call", [
+    ("layer_norm", lambda x: B.layer_norm(x)),
+    ("row_dropout", lambda x: B.dropout(x, 0.3, seed=1)),
+    ("residual_norm", lambda x: B.residual_norm(x, x, p=0.3, seed=1))])
+def test_make_fx_records_the_custom_operators(name, call):
+    with FakeTensorMode():
+        x = torch.empty(2, 8, device="cuda")
+        graph = make_fx(call)(x)
+    targets = [str(n.target) for n in graph.graph.nodes if n.op == "call_function"]
+    assert "bilinear_hip.%s.default" % name in targets and not any("empty" in t for t in targets)
+
+
+def test_a_module_that_drops_is_not_traced_with_one_mask():
+    with pytest.raises(RuntimeError, match="every call would draw the same mask"):
+        torch.jit.trace(B.Dropout(0.3), torch.ones(3))
+    with pytest.raises(RuntimeError, match="every call would draw the same mask"):
+        torch.jit.trace(B.ResidualNorm(3, p=0.3), (torch.ones(3), torch.ones(3)))
+    torch.jit.trace(B.Dropout(0.3).eval(), torch.ones(3))
