@@ -193,7 +193,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def dropout(x, p, seed, step=0, layer=0, row_offset=0, device_step=None):
     """Drop elements of ``x`` with probability ``p`` (rounded to a multiple of 2^-16) and scale the others so that the
     expectation stays; what is dropped is zero whatever it held.  The mask depends on (seed, step, layer, global row,
-    column) alone — ``row_offset`` is the global index of the first row, so a batch split over devices draws the mask of
+    column) alone — one word of the generator's key is ``seed ^ (step >> 32)``, so let steps that count stay below 2^32 where
+    several seeds are in use — ``row_offset`` is the global index of the first row, so a batch split over devices draws the mask of
     the whole one — and is drawn again in the backward pass instead of being stored.  ``device_step``: an int64 tensor
     that is added to ``step`` when the kernel runs: a captured graph that advances it draws another mask each replay."""
     if torch.compiler.is_compiling():
@@ -232,9 +233,10 @@ class _Draws:
     """The draws of a module that drops: torch's seed at the first call, a stream id that is unique in the process (a copy
     gets its own, as every stand-alone stage does) and, as the step, a number from torch's CPU generator — so
     ``torch.manual_seed`` repeats the masks, a saved generator state continues them and a checkpointed block (which
-    restores that state) is recomputed with the mask it had.  In a captured graph such a number would be frozen: give the
-    module an int64 device tensor (``set_device_step``) that the graph advances between replays.  ``row_offset``: the
-    global index of this process's first row, so that ranks with one seed draw the parts of one mask."""
+    restores that state) is recomputed with the mask it had, in a captured graph as well.  There the number is frozen: give
+    the module an int64 device tensor (``set_device_step``), which is added to it and which the graph advances between
+    replays.  ``row_offset``: the global index of this process's first row, so that ranks with one seed draw the parts of
+    one mask."""
 
     _device_step = None
     row_offset = 0
@@ -243,7 +245,7 @@ class _Draws:
         from .model.bilinear import _HeavyLinear
         self._layer = _HeavyLinear._next_stage_id[0]
         _HeavyLinear._next_stage_id[0] += 1
-        self._seed, self._captured = None, 0
+        self._seed = None
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -262,15 +264,12 @@ class _Draws:
         if torch.jit.is_tracing():
             raise RuntimeError("bilinear_amd: dropout in a trace: every call would draw the same mask.  Trace the module in "
                                "eval mode, or the function `dropout` with a device_step")
+        step, device_step = int(torch.empty((), dtype=torch.int64).random_()), None
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            if self._device_step is None:
+            device_step = self._device_step
+            if device_step is None:
                 raise RuntimeError("bilinear_amd: dropout in a stream capture needs a step on the device "
                                    "(set_device_step): every replay would draw the same mask")
-            # calls of one captured step differ in the upper half of the step, replays in the device's count
-            self._captured += 1
-            step, device_step = self._captured << 32, self._device_step
-        else:
-            step, device_step = int(torch.empty((), dtype=torch.int64).random_()), None
         return {"seed": self._seed, "step": step, "layer": self._layer, "row_offset": self.row_offset,
                 "device_step": device_step}
 

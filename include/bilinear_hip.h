@@ -502,7 +502,8 @@ typedef enum { BLH_F32 = 0, BLH_BF16 = 1, BLH_F16 = 2 } blh_dtype;
 /* Dropout of rows.  Element (i, j) is kept when a 16-bit draw u(i, j) >= t = floor(65536 p + 1/2) and then scaled by
  * 65536 / (65536 - t); else it is 0 whatever x holds.  u: Philox4x32-10, one call per 8 columns of a global row
  * (csrc/row_dropout.hip gives the counter).  The mask depends on (seed, step, layer, row_offset + i, j) alone: the
- * backward pass is the same call on dy.  It is not the mask of blh_dropout (one bit per element, p = 0.5).
+ * backward pass is the same call on dy.  One word of the key is seed ^ (step >> 32): (seed ^ d, step ^ (d << 32)) is the
+ * mask of (seed, step), so that counting steps stay below 2^32 where several seeds are in use.  It is not the mask of blh_dropout (one bit per element, p = 0.5).
  * row_offset + rows <= 2^43.                                                                                         */
 typedef struct {
   double p;                  /* 0 .. 1                                                                                */

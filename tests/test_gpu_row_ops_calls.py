@@ -172,6 +172,99 @@ def test_modules_that_drop_are_not_traced_with_one_mask(B):
         _equal(traced(*args), m(*args))
 
 
+# ---- captures -------------------------------------------------------------------------------------------------------
+
+def test_captured_modules_draw_again_what_a_restored_generator_drew(B):
+    """What a checkpointed block does: the CPU generator's state is restored and the block called again, in one capture."""
+    x = data(60, 48, F32, 1)
+    drop, norm = B.Dropout(0.4), B.ResidualNorm(48, p=0.4).cuda()
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+    drop.set_device_step(step)
+    norm.set_device_step(step)
+
+    def block():
+        return drop(x), norm(x, x)[1]
+    with torch.no_grad():
+        B.dropout(x, 0.4, seed=1, device_step=step)           # (loads the library outside the capture)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            state = torch.get_rng_state()
+            first = block()
+            torch.set_rng_state(state)
+            again = block()
+            other = block()
+            step.add_(1)
+    seen = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        _equal(again, first)
+        for p, q in zip(other, first):
+            assert not torch.equal(p, q)
+        seen.append([t.clone() for t in first])
+    for i in (1, 2):
+        for p, q in zip(seen[i], seen[0]):
+            assert not torch.equal(p, q)
+
+
+def test_a_checkpointed_block_in_a_captured_step(B):
+    """Forward, recomputation and backward in one graph: with the gradient of sum y each kept element of dx is the scale, so dx
+    shows the recomputed mask beside the forward's."""
+    from torch.utils.checkpoint import checkpoint
+    drop, x = B.Dropout(0.4), torch.ones(30, 48, device="cuda", requires_grad=True)
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+    drop.set_device_step(step)
+
+    def work():
+        state = torch.get_rng_state()
+        y = checkpoint(lambda t: _restored(drop, t, state), x, use_reentrant=False, preserve_rng_state=False)
+        return y.detach(), torch.autograd.grad(y, x, torch.ones_like(y))[0]
+
+    def _restored(m, t, state):
+        torch.set_rng_state(state)
+        return m(t).square() * 0.5                 # (reads its input in the backward: it has to be recomputed)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, dx = work()
+        step.add_(1)
+    masks = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        masks.append(y != 0)
+        assert torch.equal(dx != 0, masks[-1]) and masks[-1].any() and not masks[-1].all()
+    assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
+
+
+def test_compiled_functions_in_torchs_own_graphs(B):
+    """mode="reduce-overhead" captures the compiled calls; the step on the device moves on between them."""
+    x, dy = data(40, 96, F32, 1).requires_grad_(), data(40, 96, F32, 2)
+    w, b = params(96, F32, 5)
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+
+    def f(x, w, b, step):
+        return B.layer_norm(B.dropout(x, 0.3, 5, 7, 2, 0, step), w, b)
+    compiled = torch.compile(f, mode="reduce-overhead", fullgraph=True)
+    outs = []
+    for n in range(5):
+        torch.compiler.cudagraph_mark_step_begin()
+        y = compiled(x, w, b, step)
+        got = [y.detach().clone()] + [t.clone() for t in torch.autograd.grad(y, (x, w, b), dy)]
+        del y
+        z = f(x, w, b, step)
+        for p, q in zip(got, [z.detach(), *torch.autograd.grad(z, (x, w, b), dy)]):
+            assert torch.equal(p, q), n
+        outs.append(got[0])
+        step.add_(1)
+    assert not torch.equal(outs[3], outs[4])
+
+
 # ---- values at the ends of the range ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,width", [(2, 12), (3, 64), (1025, 64), (1026, 12), (1027, 5), (1027, 200), (2, 20004)])

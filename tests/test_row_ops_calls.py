@@ -1,4 +1,4 @@
-"""Row operators without a GPU under the calls around them: tracers and shape propagation."""
+"""Row operators without a GPU under the calls around them: tracers, shape propagation, the modules' draws."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -42,3 +42,33 @@ def test_a_module_that_drops_is_not_traced_with_one_mask():
     with pytest.raises(RuntimeError, match="every call would draw the same mask"):
         torch.jit.trace(B.ResidualNorm(3, p=0.3), (torch.ones(3), torch.ones(3)))
     torch.jit.trace(B.Dropout(0.3).eval(), torch.ones(3))
+
+
+def test_a_restored_generator_repeats_the_draws_in_a_capture(monkeypatch):
+    """(A checkpointed block, called again in the capture of its backward pass, restores the CPU generator's state.)"""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    for m in (B.Dropout(0.1), B.ResidualNorm(8, p=0.1)):
+        m.set_device_step(torch.zeros(1, dtype=torch.int64))
+        state = torch.get_rng_state()
+        first, second = m._next_draws(), m._next_draws()
+        torch.set_rng_state(state)
+        again = m._next_draws()
+        assert again["device_step"] is first["device_step"] is m._device_step
+        assert again["step"] == first["step"] and second["step"] != first["step"]
+
+
+def test_seeds_that_differ_do_not_share_masks_in_a_capture(monkeypatch):
+    """The generator's key holds seed ^ (step >> 32) in one word: steps that counted calls in those bits gave modules of two seeds
+    (ranks that seed by their index) one another's masks."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    keys = set()
+    for seed in range(8):
+        torch.manual_seed(seed)
+        m = B.Dropout(0.1)
+        m.set_device_step(torch.zeros(1, dtype=torch.int64))
+        for _ in range(8):
+            d = m._next_draws()
+            keys.add(((d["seed"] & 0xFFFFFFFF) ^ (d["step"] >> 32), d["seed"] >> 32))
+    assert len(keys) == 64
