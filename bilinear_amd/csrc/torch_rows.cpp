@@ -163,8 +163,10 @@ struct Moments {
 
 Tensor both_moments(const Tensor& x) { return at::empty({2, rows_of(x)}, x.options().dtype(at::kFloat)); }
 
-Tensor used_step(const Draws& d) {
-  return d.device_step.defined() ? at::empty({1}, d.device_step.options()) : Tensor();
+// where the kernel leaves the step that it used (a call without rows launches none)
+Tensor used_step(const Draws& d, const Tensor& x) {
+  if (!d.device_step.defined()) return Tensor();
+  return x.numel() ? at::empty({1}, d.device_step.options()) : d.device_step.add(d.step).reshape({1});
 }
 
 Tensor layer_norm_launch(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, int32_t param_code,
@@ -225,7 +227,7 @@ std::tuple<Tensor, Tensor> residual_norm_launch(const Tensor& x, const Tensor& r
   Tensor h = at::empty(x.sizes(), residual.options());
   const blh_row_drop drop = drop_of(d, used);
   check_status(blh_residual_norm_forward(stream_of(x), in.ptr(), in.ld, res.ptr(), res.ld, ptr(weight), ptr(bias), eps,
-                                         d.p > 0.0 ? &drop : nullptr, out_ptr(y), out_ptr(h), m.mean, m.rstd,
+                                         d.p > 0.0 || used.defined() ? &drop : nullptr, out_ptr(y), out_ptr(h), m.mean, m.rstd,
                                          rows_of(x), x.size(-1), code_of(x.scalar_type()),
                                          code_of(residual.scalar_type()), param_code), "blh_residual_norm_forward");
   return {y, h};
@@ -459,7 +461,7 @@ Tensor dropout(const Tensor& x, double p, int64_t seed, int64_t step, int64_t la
   if (followed({&x, &d.device_step})) return custom_dropout(x, d);
   const bool grad = wants_grad({&x});
   if (grad) refuse_eager_leaves(std::initializer_list<const Tensor*>{&x});
-  const Tensor used = grad ? used_step(d) : Tensor();
+  const Tensor used = grad ? used_step(d, x) : Tensor();
   Tensor y = dropout_launch(x, d, used);
   if (grad) {
     if (used.defined()) d.step = 0;
@@ -487,7 +489,7 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const Tensor& residual
   if (!grad) return residual_norm_launch(x, residual, dense(w), dense(b), eps, d, code, Moments(), Tensor());
   refuse_eager_leaves(std::initializer_list<const Tensor*>{&x, &residual, &w, &b});
   const Tensor both = both_moments(x);
-  const Tensor used = used_step(d);
+  const Tensor used = used_step(d, x);
   auto [y, h] = residual_norm_launch(x, residual, dense(w), dense(b), eps, d, code, Moments(both), used);
   if (used.defined()) d.step = 0;
   d.device_step = used;
@@ -551,7 +553,7 @@ std::tuple<Tensor, Tensor> op_row_dropout(const Tensor& x, double p, int64_t see
   check_rows(x, "x");
   const Draws d{p, seed, step, layer, row_offset, plain(device_step)};
   check_draws(d, x);
-  const Tensor used = used_step(d);
+  const Tensor used = used_step(d, x);
   Tensor y = dropout_launch(x, d, used);
   return {y, filled(used, x, at::kLong)};
 }
@@ -567,7 +569,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> op_residual_norm(
   check_draws(d, x);
   const auto o = x.options().dtype(at::kFloat);
   const Tensor mean = at::empty({rows_of(x)}, o), rstd = at::empty({rows_of(x)}, o);
-  const Tensor used = used_step(d);
+  const Tensor used = used_step(d, x);
   auto [y, h] = residual_norm_launch(x, residual, dense(plain(weight)), dense(plain(bias)), eps, d, code,
                                      Moments(mean, rstd), used);
   return {y, h, mean, rstd, filled(used, x, at::kLong)};

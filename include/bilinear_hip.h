@@ -511,8 +511,8 @@ typedef struct {
   int64_t row_offset;        /* global index of local row 0 (data parallel), >= 0                                     */
   const uint64_t* step_dev;  /* device, or NULL: added to `step` when the kernel runs, so that a replayed graph draws
                                 another mask each time                                                                */
-  uint64_t* step_used;       /* device, or NULL; not step_dev itself: receives step + *step_dev when anything can be dropped
-                                (t > 0), for a backward pass that runs after *step_dev has moved on                   */
+  uint64_t* step_used;       /* device, or NULL; not step_dev itself: receives step + *step_dev (if there is a row), for a
+                                backward pass that runs after *step_dev has moved on                                  */
   int32_t layer;             /* stream id, >= 0: calls that must not share a mask differ in it or in `step`           */
   int32_t reserved;
 } blh_row_drop;

@@ -265,6 +265,18 @@ def test_compiled_functions_in_torchs_own_graphs(B):
     assert not torch.equal(outs[3], outs[4])
 
 
+@pytest.mark.parametrize("p", [0.0, 1e-7, 0.3])
+@pytest.mark.parametrize("rows", [0, 3])
+def test_the_operators_return_the_step_they_used(B, p, rows):
+    op = torch.ops.bilinear_hip
+    x = torch.zeros(rows, 24, device="cuda")
+    step = torch.full((1,), 11, dtype=torch.int64, device="cuda")
+    junk = [torch.full((1,), 77, dtype=torch.int64, device="cuda") for _ in range(8)]      # what a fresh allocation may hold
+    del junk
+    assert op.row_dropout(x, p, 1, 5, 0, 0, step)[1].item() == 16
+    assert op.residual_norm(x, x, None, None, 1e-5, p, 1, 5, 0, 0, step)[4].item() == 16
+
+
 # ---- values at the ends of the range ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,width", [(2, 12), (3, 64), (1025, 64), (1026, 12), (1027, 5), (1027, 200), (2, 20004)])
