@@ -375,13 +375,17 @@ Tensor dropout(const Tensor& x, double p, int64_t seed, int64_t step, int64_t la
                const Optional& device_step);
 
 // dropout is linear: its backward is the same map, with the same derivative
+Tensor dropped(const Tensor& dy, const Draws& d) {
+  if (!at::GradMode::is_enabled() && !followed({&dy})) return dropout_launch(dy, d, Tensor());
+  return dropout(dy, d.p, d.seed, d.step, d.layer, d.row_offset, given(d.device_step));
+}
+
 struct RowDropoutBackward : public torch::autograd::Node {
   Draws d;
   std::string name() const override { return "BilinearRowDropoutBackward"; }
   variable_list apply(variable_list&& grads) override {
     if (!grads[0].defined()) return variable_list(1);
-    if (!at::GradMode::is_enabled() && !followed({&grads[0]})) return {dropout_launch(grads[0], d, Tensor())};
-    return {dropout(grads[0], d.p, d.seed, d.step, d.layer, d.row_offset, given(d.device_step))};
+    return {dropped(grads[0], d)};
   }
 };
 
@@ -401,15 +405,21 @@ struct ResidualNormBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(4);
-    const Tensor stream = h.unpack(shared_from_this()), w = weight.unpack();
-    // only the stream went on: the norm's share is zero
-    const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(stream.sizes(), stream.options().dtype(dtype));
     const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1),
                need_w = task_should_compute_output(2), need_b = task_should_compute_output(3);
+    const bool drops = (int64_t)(d.p * 65536.0 + 0.5) != 0;
+    if (!grads[0].defined()) {
+      // only the stream went on: the sum's gradients, whatever the rows' statistics are (a row may hold an infinity)
+      const Tensor& dh = grads[1];
+      const auto o = dh.options().dtype(code == BLH_F32 ? at::kFloat : dtype);
+      return {need_x ? (drops ? dropped(dh, d) : dh).to(dtype) : Tensor(), wanted(need_r, dh),
+              need_w ? at::zeros({dh.size(-1)}, o) : Tensor(), need_b ? at::zeros({dh.size(-1)}, o) : Tensor()};
+    }
+    const Tensor &dy = grads[0], stream = h.unpack(shared_from_this()), w = weight.unpack();
     if (followed({&dy, &grads[1], &stream, &w}))
       return custom_residual_norm_backward(dy, grads[1], stream, w, moments, d, need_x, need_r, need_w, need_b, code);
     // without dropout and with one type both branches of the sum get the same gradient: it is written once
-    const bool same = need_x && need_r && stream.scalar_type() == dtype && (int64_t)(d.p * 65536.0 + 0.5) == 0;
+    const bool same = need_x && need_r && stream.scalar_type() == dtype && !drops;
     variable_list out = residual_norm_backward_launch(dy, grads[1], stream, dense(w), Moments(moments), d, need_x && !same,
                                                       need_r, need_w, need_b, code);
     if (same) out[0] = out[1];

@@ -157,14 +157,22 @@ def _res_setup(ctx, inputs, output):
     _refuse_eager_leaves(inputs)
     x, residual, weight, bias, _, p, seed, step, layer, row_offset, device_step = inputs
     ctx.mark_non_differentiable(*output[2:])
+    ctx.set_materialize_grads(False)
     ctx.save_for_backward(output[1], weight, output[2], output[3], None if device_step is None else output[4])
     ctx.draws = (p, seed, step if device_step is None else 0, layer, row_offset)
-    ctx.code = _param_code(x, weight, bias)
+    ctx.code, ctx.dtype = _param_code(x, weight, bias), x.dtype
 
 
 def _res_formula(ctx, dy, dh, *unused):
     h, weight, mean, rstd, used = ctx.saved_tensors
     need = ctx.needs_input_grad[:4]
+    if dy is None:
+        if dh is None:
+            return (None,) * 11
+        # only the stream went on: the sum's gradients, whatever the rows' statistics are
+        dx = torch.ops.bilinear_hip.row_dropout(dh, *ctx.draws, used)[0] if int(ctx.draws[0] * 65536 + 0.5) else dh
+        zeros = dh.new_zeros(dh.shape[-1], dtype=torch.float32 if ctx.code == 0 else ctx.dtype)
+        return _pick(need, (dx.to(ctx.dtype), dh, zeros, zeros.clone())) + (None,) * 7
     return _pick(need, torch.ops.bilinear_hip.residual_norm_backward(
         dy, dh, h, weight, mean, rstd, *ctx.draws, used, *need, ctx.code)) + (None,) * 7
 

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import row_ops_util as R
-from test_gpu_row_ops import BF16, F32, d, data, params
+from test_gpu_row_ops import BF16, F16, F32, d, data, params
 
 pytestmark = pytest.mark.gpu
 
@@ -21,15 +21,14 @@ def _first_outputs(B):
     return {
         "layer_norm": lambda x, r, w, b: B.layer_norm(x, w, b),
         "residual_norm": lambda x, r, w, b: B.residual_norm(x, r, w, b, p=0.3, seed=1)[0],
-        "residual_norm's stream": lambda x, r, w, b: B.residual_norm(x, r, w, b, p=0.3, seed=1)[1],
         "residual_norm without dropout": lambda x, r, w, b: B.residual_norm(x, r, w, b)[0],
         "operator layer_norm": lambda x, r, w, b: op.layer_norm(x, w, b, 1e-5)[0],
         "operator residual_norm": lambda x, r, w, b: op.residual_norm(x, r, w, b, 1e-5, 0.3, 1, 0, 0, 0, None)[0],
     }
 
 
-@pytest.mark.parametrize("name", ["layer_norm", "residual_norm", "residual_norm's stream", "residual_norm without dropout",
-                                  "operator layer_norm", "operator residual_norm"])
+@pytest.mark.parametrize("name", ["layer_norm", "residual_norm", "residual_norm without dropout", "operator layer_norm",
+                                  "operator residual_norm"])
 def test_a_second_derivative_is_refused_beside_other_terms(B, name):
     """A gradient penalty in a loss that has other gradients: its share must not be dropped in silence."""
     x, r = data(3, 16, F32, 1).requires_grad_(), data(3, 16, F32, 2).requires_grad_()
@@ -71,6 +70,21 @@ def test_second_derivative_of_dropout(B, operator, device_step):
     f = R.factor(20, 40, 0.3, seed=7, step=5, layer=2, row_offset=3)
     want = 36 * f ** 6 * d(x) ** 3 + f
     R.close(got, want, 24 * R.U * (36 * f ** 6 * d(x).abs() ** 3 + f) + R.tiny(F32), "second derivative")
+
+
+@pytest.mark.parametrize("operator", [False, True])
+def test_second_derivative_of_the_stream(B, operator):
+    """h = r + f x, g = d(sum h^3)/dx = 3 f h^2, d(sum g^2)/dx = 36 f^3 h^3.  h is off by U |h|, the rest by some fifteen roundings
+    more."""
+    x, r = data(9, 40, F32, 1).requires_grad_(), data(9, 40, F32, 2).requires_grad_()
+    w, b = params(40, F32, 5)
+    h = (torch.ops.bilinear_hip.residual_norm(x, r, w, b, 1e-5, 0.3, 7, 0, 0, 0, None) if operator
+         else B.residual_norm(x, r, w, b, p=0.3, seed=7))[1]
+    g, = torch.autograd.grad(h.pow(3).sum(), x, create_graph=True)
+    got, = torch.autograd.grad(g.square().sum(), x)
+    f = R.factor(9, 40, 0.3, seed=7)
+    want = 36 * f ** 3 * (d(r) + f * d(x)) ** 3
+    R.close(got, want, 28 * R.U * want.abs() + R.tiny(F32), "second derivative")
 
 
 # ---- tracers --------------------------------------------------------------------------------------------------------
@@ -308,3 +322,22 @@ def test_a_mean_times_rstd_past_the_largest_number(B, rows, width, dtype):
     want = (D[:-1] * R.norm64(X, Wt, Bi, eps)[3]).sum(0)
     R.close(dw, want, R.rounded(e_dw, want, F32), "dw")
     R.close(db, D.sum(0), R.rounded(e_db + 400 * R.U * D[-1].abs(), D.sum(0), F32), "db")
+
+
+@pytest.mark.parametrize("operator", [False, True])
+@pytest.mark.parametrize("dtype,rtype,p", [(F32, F32, 0.0), (F32, F32, 0.3), (BF16, F32, 0.3), (BF16, BF16, 0.0), (F16, F32, 0.0)])
+def test_the_stream_alone_carries_its_gradient_past_a_row_without_statistics(B, operator, dtype, rtype, p):
+    """Only h goes on: dresidual = dh and dx = dropout(dh), whatever the norm of that row would have been."""
+    x, r, dh = data(5, 40, dtype, 1), data(5, 40, rtype, 2), data(5, 40, rtype, 3)
+    x[1, 4], r[2, 5], r[3, 6] = float("inf"), float("nan"), float("-inf")
+    x.requires_grad_(), r.requires_grad_()
+    w, b = params(40, F32, 5)
+    if operator:
+        h = torch.ops.bilinear_hip.residual_norm(x, r, w, b, 1e-5, p, 9, 0, 0, 0, None)[1]
+    else:
+        h = B.residual_norm(x, r, w, b, p=p, seed=9)[1]
+    dx, dr, dw, db = torch.autograd.grad(h, (x, r, w, b), dh)
+    f = R.factor(5, 40, p, seed=9) if p else torch.ones(5, 40, dtype=torch.double)
+    assert torch.equal(dr, dh)
+    assert torch.equal(dx.cpu(), (d(dh) * f).float().to(dtype))
+    assert dw.dtype == db.dtype == F32 and not dw.any() and not db.any()
