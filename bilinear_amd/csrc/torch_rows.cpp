@@ -319,12 +319,20 @@ variable_list custom_residual_norm_backward(const Tensor& dy, const Tensor& dh, 
 
 // A leaf's gradient accumulator belongs to the stream it was made on.  One that an eager graph on the DEFAULT stream still
 // holds cannot take part in a stream capture (that stream cannot be captured: the capture would break inside the autograd
-// engine, where the error ends the process), so such a call is refused before anything is enqueued.
+// engine, where the error ends the process), so such a call is refused before anything is enqueued.  A view's leaf is its base.
 template <typename L> void refuse_eager_leaves(const L& inputs) {
+  c10::OptionalDeviceGuard guard;
+  for (const Tensor* t : inputs) {
+    if (!t->defined()) continue;
+    guard.reset_device(t->device());      // (the inputs' one device, which need not be the current one)
+    break;
+  }
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   for (const Tensor* t : inputs) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!t->defined() || !t->requires_grad()) continue;
+    const Tensor leaf = !t->is_leaf() && t->is_view() ? Tensor(t->_base()) : *t;
+    if (!leaf.requires_grad() || !leaf.is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
     if (!node) continue;
     const auto s = node->stream();
     TORCH_CHECK(!s || s->id() != 0,

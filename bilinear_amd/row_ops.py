@@ -120,9 +120,19 @@ def _pick(needed, grads):
     return tuple(g if n else None for n, g in zip(needed, grads))
 
 
+def _capturing(x):
+    """Whether the current stream of x's device, where the kernels go, is being captured."""
+    if not torch.cuda.is_available():
+        return False
+    if x is None or x.device.index is None or x.device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(x.device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _refuse_eager_leaves(inputs):
     """In a stream capture: what the functions refuse (csrc/torch_rows.cpp), for calls of the operators themselves."""
-    if not torch.compiler.is_compiling() and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+    if not torch.compiler.is_compiling() and _capturing(inputs[0]):
         _native().refuse_eager_leaves([t for t in inputs if isinstance(t, torch.Tensor)])
 
 
@@ -266,14 +276,14 @@ class _Draws:
             raise RuntimeError("the device step is one int64")
         self._device_step = tensor
 
-    def _next_draws(self):
+    def _next_draws(self, x=None):
         if self._seed is None:
             self._seed = int(torch.initial_seed()) & ((1 << 63) - 1)
         if torch.jit.is_tracing():
             raise RuntimeError("bilinear_amd: dropout in a trace: every call would draw the same mask.  Trace the module in "
                                "eval mode, or the function `dropout` with a device_step")
         step, device_step = int(torch.empty((), dtype=torch.int64).random_()), None
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        if _capturing(x):
             device_step = self._device_step
             if device_step is None:
                 raise RuntimeError("bilinear_amd: dropout in a stream capture needs a step on the device "
@@ -294,7 +304,7 @@ class Dropout(_Draws, nn.Dropout):
     def forward(self, x):
         if not self.training or self.p == 0.0:
             return x
-        return dropout(x, self.p, **self._next_draws())
+        return dropout(x, self.p, **self._next_draws(x))
 
 
 class ResidualNorm(_Draws, nn.LayerNorm):
@@ -316,5 +326,5 @@ class ResidualNorm(_Draws, nn.LayerNorm):
     def forward(self, x, residual):
         if x.dim() < 1 or x.shape[-1] != self.normalized_shape[0]:
             raise RuntimeError("expected rows of %d columns, got shape %s" % (self.normalized_shape[0], tuple(x.shape)))
-        draws = self._next_draws() if self.training and self.p else {}
+        draws = self._next_draws(x) if self.training and self.p else {}
         return residual_norm(x, residual, self.weight, self.bias, self.eps, self.p if draws else 0.0, **draws)

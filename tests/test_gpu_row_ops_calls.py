@@ -291,6 +291,21 @@ def test_the_operators_return_the_step_they_used(B, p, rows):
     assert op.residual_norm(x, x, None, None, 1e-5, p, 1, 5, 0, 0, step)[4].item() == 16
 
 
+def test_a_view_of_a_leaf_of_a_live_eager_graph_is_refused_in_a_capture(B):
+    x = data(8, 16, F32, 1)
+    w = params(32, F32, 5)[0]
+    eager = B.layer_norm(x, w[:16])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="still part of an eager autograd graph"):
+            B.layer_norm(x, w[:16])
+        with torch.no_grad():
+            z = B.layer_norm(x, w[:16])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(z, eager)
+
+
 # ---- values at the ends of the range ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,width", [(2, 12), (3, 64), (1025, 64), (1026, 12), (1027, 5), (1027, 200), (2, 20004)])

@@ -1,4 +1,6 @@
 """Row operators without a GPU under the calls around them: tracers, shape propagation, the modules' draws."""
+import types
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -72,3 +74,27 @@ def test_seeds_that_differ_do_not_share_masks_in_a_capture(monkeypatch):
             d = m._next_draws()
             keys.add(((d["seed"] & 0xFFFFFFFF) ^ (d["step"] >> 32), d["seed"] >> 32))
     assert len(keys) == 64
+
+
+def test_the_capture_that_counts_is_that_of_the_inputs_device(monkeypatch):
+    """(Stands in for two devices: the stream of device 1 is captured, device 0 is the current one.)"""
+    current = [0]
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == 1)
+    m = B.Dropout(0.1)
+    m.set_device_step(torch.zeros(1, dtype=torch.int64))
+    there, here = (types.SimpleNamespace(device=torch.device("cuda", i)) for i in (1, 0))
+    assert m._next_draws(there)["device_step"] is m._device_step and m._next_draws(here)["device_step"] is None
+    assert current == [0]
