@@ -112,6 +112,14 @@ void check_status(int status, const char* what) {
 // What a kernel may read: a lazily negated view (an imaginary part of a conjugate) is resolved first.
 Tensor readable(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 
+// NULL says that a tensor was left out: one whose storage has been freed (a sharded parameter, say) is not that.
+const void* address(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  TORCH_CHECK(t.numel() == 0 || t.storage().nbytes() != 0, "bilinear_amd row operators: a tensor of shape ", t.sizes(),
+              " has no storage");
+  return t.const_data_ptr();
+}
+
 // Rows are read in place where the last axis is dense and the leading axes collapse to one, else from a dense copy.
 struct Rows {
   Tensor t;
@@ -137,19 +145,18 @@ struct Rows {
     }
     t = x.contiguous();
   }
-  const void* ptr() const { return t.defined() ? t.const_data_ptr() : nullptr; }
+  const void* ptr() const { return address(t); }
 };
 
 Tensor dense(const Tensor& t) { return t.defined() ? readable(t).contiguous() : t; }
 Tensor plain(const Optional& t) { return t ? *t : Tensor(); }
-const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 void* stream_of(const Tensor& x) { return (void*)c10::hip::getCurrentHIPStream(x.get_device()).stream(); }
 int64_t rows_of(const Tensor& x) { return x.numel() / x.size(-1); }
 
 blh_row_drop drop_of(const Draws& d, const Tensor& used) {
   return blh_row_drop{d.p, (uint64_t)d.seed, (uint64_t)d.step, d.row_offset,
-                      (const uint64_t*)ptr(d.device_step), (uint64_t*)out_ptr(used), (int32_t)d.layer, 0};
+                      (const uint64_t*)address(d.device_step), (uint64_t*)out_ptr(used), (int32_t)d.layer, 0};
 }
 
 // what the backward reads of the forward, [rows] each (both NULL: not kept)
@@ -174,7 +181,7 @@ Tensor layer_norm_launch(const Tensor& x, const Tensor& weight, const Tensor& bi
   const c10::OptionalDeviceGuard guard(x.device());
   const Rows in(x);
   Tensor y = at::empty(x.sizes(), x.options());
-  check_status(blh_layer_norm_forward(stream_of(x), in.ptr(), in.ld, ptr(weight), ptr(bias), eps, out_ptr(y), m.mean,
+  check_status(blh_layer_norm_forward(stream_of(x), in.ptr(), in.ld, address(weight), address(bias), eps, out_ptr(y), m.mean,
                                       m.rstd, rows_of(x), x.size(-1), code_of(x.scalar_type()), param_code),
                "blh_layer_norm_forward");
   return y;
@@ -201,7 +208,7 @@ variable_list layer_norm_backward_launch(const Tensor& dy, const Tensor& x, cons
   const Rows gy(dy), in(x);
   Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : Tensor();
   const ParamGrads g(x, need_weight, need_bias, code);
-  check_status(blh_layer_norm_backward(stream_of(x), gy.ptr(), gy.ld, in.ptr(), in.ld, ptr(weight), m.mean, m.rstd,
+  check_status(blh_layer_norm_backward(stream_of(x), gy.ptr(), gy.ld, in.ptr(), in.ld, address(weight), m.mean, m.rstd,
                                        out_ptr(dx), out_ptr(g.weight), out_ptr(g.bias), out_ptr(g.workspace), g.bytes(),
                                        rows_of(x), x.size(-1), code_of(x.scalar_type()), code),
                "blh_layer_norm_backward");
@@ -226,7 +233,7 @@ std::tuple<Tensor, Tensor> residual_norm_launch(const Tensor& x, const Tensor& r
   Tensor y = at::empty(x.sizes(), x.options());
   Tensor h = at::empty(x.sizes(), residual.options());
   const blh_row_drop drop = drop_of(d, used);
-  check_status(blh_residual_norm_forward(stream_of(x), in.ptr(), in.ld, res.ptr(), res.ld, ptr(weight), ptr(bias), eps,
+  check_status(blh_residual_norm_forward(stream_of(x), in.ptr(), in.ld, res.ptr(), res.ld, address(weight), address(bias), eps,
                                          d.p > 0.0 || used.defined() ? &drop : nullptr, out_ptr(y), out_ptr(h), m.mean, m.rstd,
                                          rows_of(x), x.size(-1), code_of(x.scalar_type()),
                                          code_of(residual.scalar_type()), param_code), "blh_residual_norm_forward");
@@ -243,7 +250,7 @@ variable_list residual_norm_backward_launch(const Tensor& dy, const Tensor& dh, 
   Tensor dres = need_residual ? at::empty(h.sizes(), h.options()) : Tensor();
   const ParamGrads g(dy, need_weight, need_bias, code);
   const blh_row_drop drop = drop_of(d, Tensor());
-  check_status(blh_residual_norm_backward(stream_of(h), gy.ptr(), gy.ld, gh.ptr(), gh.ld, in.ptr(), in.ld, ptr(weight),
+  check_status(blh_residual_norm_backward(stream_of(h), gy.ptr(), gy.ld, gh.ptr(), gh.ld, in.ptr(), in.ld, address(weight),
                                           m.mean, m.rstd, d.p > 0.0 ? &drop : nullptr, out_ptr(dx), out_ptr(dres),
                                           out_ptr(g.weight), out_ptr(g.bias), out_ptr(g.workspace), g.bytes(), rows_of(h),
                                           h.size(-1), code_of(dy.scalar_type()), code_of(h.scalar_type()), code),

@@ -356,3 +356,14 @@ def test_the_stream_alone_carries_its_gradient_past_a_row_without_statistics(B, 
     assert torch.equal(dr, dh)
     assert torch.equal(dx.cpu(), (d(dh) * f).float().to(dtype))
     assert dw.dtype == db.dtype == F32 and not dw.any() and not db.any()
+
+
+def test_tensors_whose_storage_is_gone_are_refused(B):
+    """(A parameter that a sharding library has freed is not a parameter that was left out.)"""
+    x = data(4, 16, F32, 1).contiguous()
+    gone = torch.ones(16, device="cuda")
+    gone.untyped_storage().resize_(0)
+    for call in (lambda: B.layer_norm(x, gone), lambda: B.layer_norm(x, None, gone), lambda: B.residual_norm(x, x, gone),
+                 lambda: torch.ops.bilinear_hip.layer_norm(x, gone, None, 1e-5)):
+        with pytest.raises(RuntimeError, match="no storage"):
+            call()
