@@ -1,4 +1,7 @@
 """Row operators without a GPU under the calls around them: tracers, shape propagation, the modules' draws."""
+import os
+import subprocess
+import sys
 import types
 
 import pytest
@@ -98,3 +101,12 @@ def test_the_capture_that_counts_is_that_of_the_inputs_device(monkeypatch):
     there, here = (types.SimpleNamespace(device=torch.device("cuda", i)) for i in (1, 0))
     assert m._next_draws(there)["device_step"] is m._device_step and m._next_draws(here)["device_step"] is None
     assert current == [0]
+
+
+def test_the_c_library_builds_without_pytorch():
+    csrc = os.path.join(os.path.dirname(B.__file__), "csrc")
+
+    def commands(*args):
+        return subprocess.run(["make", "-n", "-B", "-C", csrc, "all", *args], capture_output=True, text=True, check=True).stdout
+    with_torch, without = commands("PYTHON=" + sys.executable), commands("PYTHON=false")
+    assert "libbilinear_hip.so" in without and "torch_rows" not in without and "torch_rows" in with_torch
