@@ -5,13 +5,12 @@
 // and autograd runs a backward node on its device thread, where a Python node starts with cold caches.  Measured with
 // ctypes and a Python autograd.Function: forward + backward of a 64 x 1024 layer norm 143 us, without a gradient 12.6; with
 // these nodes 40-64 us (23.6 with single-threaded autograd; the kernels are 8) and 4.3-5.
-#include <ATen/TracerMode.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
@@ -20,6 +19,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/library.h>
 
 #include <optional>
 #include <tuple>
@@ -115,9 +115,10 @@ Tensor readable(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 // NULL says that a tensor was left out: one whose storage has been freed (a sharded parameter, say) is not that.
 const void* address(const Tensor& t) {
   if (!t.defined()) return nullptr;
-  TORCH_CHECK(t.numel() == 0 || t.storage().nbytes() != 0, "bilinear_amd row operators: a tensor of shape ", t.sizes(),
-              " has no storage");
-  return t.const_data_ptr();
+  const void* p = t.const_data_ptr();           // (the offset alone where there is no storage)
+  if ((!p || t.storage_offset() != 0) && t.numel() != 0)
+    TORCH_CHECK(t.storage().nbytes() != 0, "bilinear_amd row operators: a tensor of shape ", t.sizes(), " has no storage");
+  return p;
 }
 
 // Rows are read in place where the last axis is dense and the leading axes collapse to one, else from a dense copy.
@@ -259,15 +260,16 @@ variable_list residual_norm_backward_launch(const Tensor& dy, const Tensor& dh, 
 }
 
 // ---- through the dispatcher -------------------------------------------------------------------------------------------
-// A tracer, a dispatch mode or a tensor subclass sees what goes through torch's dispatcher.  The calls below do not — it would
-// see an allocation and nothing that fills it — so that where one is present the custom operators (row_ops.py) take their
-// place: outputs that were not asked for come back empty there, and autograd is the operators' own.
+// A tracer, a dispatch mode or a tensor subclass sees what goes through torch's dispatcher.  Of the launches above that is an
+// allocation and nothing that fills it, so where one is present the custom operators (row_ops.py) take their place, with
+// their own autograd.
 
 bool followed(std::initializer_list<const Tensor*> inputs) {
-  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::dispatch_mode_enabled()) return true;
+  const auto here = c10::impl::tls_local_dispatch_key_set();
+  c10::DispatchKeySet keys = here.included_;           // (a dispatch mode sets the Python key, a tracer its own)
   for (const Tensor* t : inputs)
-    if (t->defined() && t->key_set().has(c10::DispatchKey::Python)) return true;
-  return false;
+    if (t->defined()) keys = keys | t->key_set();
+  return (keys - here.excluded_).has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Tracer}));
 }
 
 template <typename Signature> c10::TypedOperatorHandle<Signature> custom(const char* name) {
@@ -283,11 +285,14 @@ std::tuple<Tensor, Tensor, Tensor> custom_layer_norm(const Tensor& x, const Tens
   return op.call(x, given(w), given(b), eps);
 }
 
+auto layer_norm_backward_operator() {
+  return custom<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Optional&, const Tensor&, const Tensor&,
+                                                   bool, bool, bool, int64_t)>("bilinear_hip::layer_norm_backward");
+}
+
 variable_list custom_layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& moments,
                                          bool need_x, bool need_weight, bool need_bias, int64_t code) {
-  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor>(
-      const Tensor&, const Tensor&, const Optional&, const Tensor&, const Tensor&, bool, bool, bool, int64_t)>(
-      "bilinear_hip::layer_norm_backward");
+  static const auto op = layer_norm_backward_operator();
   const auto [dx, dw, db] = op.call(dy, x, given(w), moments.select(0, 0), moments.select(0, 1), need_x, need_weight,
                                     need_bias, code);
   return {wanted(need_x, dx), wanted(need_weight, dw), wanted(need_bias, db)};
@@ -309,13 +314,17 @@ std::tuple<Tensor, Tensor> custom_residual_norm(const Tensor& x, const Tensor& r
   return {std::get<0>(out), std::get<1>(out)};
 }
 
-variable_list custom_residual_norm_backward(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w,
-                                            const Tensor& moments, const Draws& d, bool need_x, bool need_residual,
-                                            bool need_weight, bool need_bias, int64_t code) {
-  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+auto residual_norm_backward_operator() {
+  return custom<std::tuple<Tensor, Tensor, Tensor, Tensor>(
       const Tensor&, const Optional&, const Tensor&, const Optional&, const Tensor&, const Tensor&, double, c10::SymInt,
       c10::SymInt, c10::SymInt, c10::SymInt, const Optional&, bool, bool, bool, bool, int64_t)>(
       "bilinear_hip::residual_norm_backward");
+}
+
+variable_list custom_residual_norm_backward(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w,
+                                            const Tensor& moments, const Draws& d, bool need_x, bool need_residual,
+                                            bool need_weight, bool need_bias, int64_t code) {
+  static const auto op = residual_norm_backward_operator();
   const auto [dx, dres, dw, db] = op.call(dy, given(dh), h, given(w), moments.select(0, 0), moments.select(0, 1), d.p, d.seed,
                                           d.step, d.layer, d.row_offset, given(d.device_step), need_x, need_residual,
                                           need_weight, need_bias, code);
@@ -361,6 +370,49 @@ variable_list once(variable_list grads) {
   const auto error = std::make_shared<torch::autograd::DelayedError>(
       "bilinear_amd row operators: trying to differentiate the backward pass, which is not supported", (int64_t)grads.size());
   return (*error)(std::move(grads));
+}
+
+void refuse_tangents(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                "bilinear_amd row operators have no forward-mode derivative");
+}
+
+bool any_needs_grad(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// The custom backward operators under autograd: the same refusals.  (In C++: as a Python formula they cost 3 us a call.)
+std::tuple<Tensor, Tensor, Tensor> autograd_layer_norm_backward(c10::DispatchKeySet keys, const Tensor& dy,
+                                                                const Tensor& x, const Optional& weight, const Tensor& mean,
+                                                                const Tensor& rstd, bool need_x, bool need_weight,
+                                                                bool need_bias, int64_t code) {
+  static const auto op = layer_norm_backward_operator();
+  const Tensor w = plain(weight);
+  refuse_tangents({&dy, &x, &w, &mean, &rstd});
+  const bool refuse = any_needs_grad({&dy, &x, &w, &mean, &rstd});
+  auto out = op.redispatch(keys & c10::after_autograd_keyset, dy, x, weight, mean, rstd, need_x, need_weight, need_bias, code);
+  if (!refuse) return out;
+  const variable_list g = once({std::get<0>(out), std::get<1>(out), std::get<2>(out)});
+  return {g[0], g[1], g[2]};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> autograd_residual_norm_backward(
+    c10::DispatchKeySet keys, const Tensor& dy, const Optional& dh, const Tensor& h, const Optional& weight,
+    const Tensor& mean, const Tensor& rstd, double p, c10::SymInt seed, c10::SymInt step, c10::SymInt layer,
+    c10::SymInt row_offset, const Optional& device_step, bool need_x, bool need_residual, bool need_weight, bool need_bias,
+    int64_t code) {
+  static const auto op = residual_norm_backward_operator();
+  const Tensor w = plain(weight), s = plain(dh);
+  refuse_tangents({&dy, &s, &h, &w, &mean, &rstd});
+  const bool refuse = any_needs_grad({&dy, &s, &h, &w, &mean, &rstd});
+  auto out = op.redispatch(keys & c10::after_autograd_keyset, dy, dh, h, weight, mean, rstd, p, seed, step, layer, row_offset,
+                           device_step, need_x, need_residual, need_weight, need_bias, code);
+  if (!refuse) return out;
+  const variable_list g = once({std::get<0>(out), std::get<1>(out), std::get<2>(out), std::get<3>(out)});
+  return {g[0], g[1], g[2], g[3]};
 }
 
 struct LayerNormBackward : public torch::autograd::Node {
@@ -447,13 +499,8 @@ template <typename N> std::shared_ptr<N> make_node() {
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> inputs) {
-  for (const Tensor* t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
-                                "bilinear_amd row operators have no forward-mode derivative");
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : inputs)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
+  refuse_tangents(inputs);
+  return at::GradMode::is_enabled() && any_needs_grad(inputs);
 }
 
 // ---- what Python calls ----------------------------------------------------------------------------------------------
@@ -620,6 +667,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_residual_norm_backward(
 }
 
 }  // namespace
+
+TORCH_LIBRARY_IMPL(bilinear_hip, AutogradCUDA, m) {
+  m.impl("layer_norm_backward", &autograd_layer_norm_backward);
+  m.impl("residual_norm_backward", &autograd_residual_norm_backward);
+}
 
 PYBIND11_MODULE(_rows, m) {
   const auto release = pybind11::call_guard<pybind11::gil_scoped_release>();

@@ -187,15 +187,9 @@ def _res_formula(ctx, dy, dh, *unused):
         dy, dh, h, weight, mean, rstd, *ctx.draws, used, *need, ctx.code)) + (None,) * 7
 
 
-def _not_twice(ctx, *grads):
-    raise RuntimeError("bilinear_amd row operators: trying to differentiate the backward pass, which is not supported")
-
-
 torch.library.register_autograd("bilinear_hip::layer_norm", _ln_formula, setup_context=_ln_setup, lib=_LIB)
 torch.library.register_autograd("bilinear_hip::row_dropout", _drop_formula, setup_context=_drop_setup, lib=_LIB)
 torch.library.register_autograd("bilinear_hip::residual_norm", _res_formula, setup_context=_res_setup, lib=_LIB)
-torch.library.register_autograd("bilinear_hip::layer_norm_backward", _not_twice, lib=_LIB)
-torch.library.register_autograd("bilinear_hip::residual_norm_backward", _not_twice, lib=_LIB)
 
 
 # ---- functions ------------------------------------------------------------------------------------------------------

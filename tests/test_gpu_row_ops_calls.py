@@ -54,6 +54,16 @@ def test_the_backward_operators_refuse_to_be_differentiated(B):
         (dx.sum() + dy.sum()).backward()
 
 
+def test_the_backward_operators_refuse_tangents(B):
+    import torch.autograd.forward_ad as fwd
+    x, w = data(3, 16, F32, 1), params(16, F32, 5)[0].detach()
+    _, mean, rstd = torch.ops.bilinear_hip.layer_norm(x, w, None, 1e-5)
+    with fwd.dual_level():
+        dual = fwd.make_dual(data(3, 16, F32, 2), data(3, 16, F32, 3))
+        with pytest.raises(NotImplementedError):
+            torch.ops.bilinear_hip.layer_norm_backward(dual, x, w, mean, rstd, True, True, True, 0)
+
+
 @pytest.mark.parametrize("operator", [False, True])
 @pytest.mark.parametrize("device_step", [False, True])
 def test_second_derivative_of_dropout(B, operator, device_step):
