@@ -28,6 +28,14 @@ int row_make_drop(const blh_row_drop* d, int64_t rows, RowDrop* out) {
   return BLH_OK;
 }
 
+__global__ void row_write_step_kernel(RowDrop drop) { row_key(drop); }
+
+int row_write_step(hipStream_t s, const RowDrop& drop) {
+  hipLaunchKernelGGL(row_write_step_kernel, dim3(1), dim3(1), 0, s, drop);
+  BLH_HIP_TRY(hipGetLastError());
+  return BLH_OK;
+}
+
 // I: the type that counts units: 32 bits wherever they fit, since the index costs a division by `units` (65536 x 64 bf16 5.4
 // against 5.8 us)
 template <typename T, typename I, bool SHORT>

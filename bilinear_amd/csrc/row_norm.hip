@@ -50,7 +50,7 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
 template <typename T, typename R, bool RESID>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormFwd p) {
   __shared__ float sh[4];
-  const RowKey key = RESID && (p.drop.threshold || p.drop.step_used) ? row_key(p.drop) : RowKey{};
+  const RowKey key = RESID && p.drop.threshold ? row_key(p.drop) : RowKey{};
   const int W = (int)p.width, units = (W + ROW_UNIT - 1) / ROW_UNIT;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(BLOCK) void norm_fwd_rows_kernel(NormFwd p) {
   constexpr int GROUPS = BLOCK / LANES;
   __shared__ float2 sh[2][16];
   RowGroup<LANES> group;
-  const RowKey key = RESID && (p.drop.threshold || p.drop.step_used) ? row_key(p.drop) : RowKey{};
+  const RowKey key = RESID && p.drop.threshold ? row_key(p.drop) : RowKey{};
   const int W = (int)p.width, lane = threadIdx.x % LANES;
   int g = threadIdx.x / LANES;
   if constexpr (LANES == 64) g = __builtin_amdgcn_readfirstlane(g);
@@ -710,6 +710,7 @@ int blh_residual_norm_forward(void* stream, const void* x, int64_t ldx, const vo
     return BLH_ERR_INVALID_ARGUMENT;
   const NormFwd p{x, residual, weight, bias, y, h, mean, rstd, ldx, ldr, rows, width, (float)eps,
                   param_dtype == dtype, d};
+  if (d.step_used && !d.threshold) BLH_TRY(row_write_step((hipStream_t)stream, d));
   return resid_fwd((hipStream_t)stream, p, dtype, stream_dtype);
 }
 

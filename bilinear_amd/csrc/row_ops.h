@@ -21,5 +21,8 @@ static inline int row_check_shape(int64_t rows, int64_t width) {
 struct RowDrop;
 // threshold = floor(65536 p + 1/2), scale = 65536 / (65536 - threshold); refuses p outside [0, 1] and rows past 2^43
 int row_make_drop(const blh_row_drop* d, int64_t rows, RowDrop* out);
+// *step_used = step + *step_dev, for a call whose kernel drops nothing and so does not look (in that kernel the write costs
+// registers: 4096 x 5000 fp16 residual norm on an fp32 stream 51.1 against 48.5 us)
+int row_write_step(hipStream_t s, const RowDrop& drop);
 
 }  // namespace blh

@@ -149,8 +149,8 @@ template <typename T> __device__ __forceinline__ void settle(RawUnit<T>& r, int 
 template <typename T, typename R> __device__ __forceinline__ void settle2(RawUnit<T>& d, RawUnit<R>& f, int c, int width) {
   if (c + ROW_UNIT > width) {
     if (c < width) {
-      d.shift(c + ROW_UNIT - width);
       f.rotate(c + ROW_UNIT - width);
+      d.shift(c + ROW_UNIT - width);
     } else {
       d.zero();
     }
