@@ -285,14 +285,11 @@ std::tuple<Tensor, Tensor, Tensor> custom_layer_norm(const Tensor& x, const Tens
   return op.call(x, given(w), given(b), eps);
 }
 
-auto layer_norm_backward_operator() {
-  return custom<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Optional&, const Tensor&, const Tensor&,
-                                                   bool, bool, bool, int64_t)>("bilinear_hip::layer_norm_backward");
-}
-
 variable_list custom_layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& moments,
                                          bool need_x, bool need_weight, bool need_bias, int64_t code) {
-  static const auto op = layer_norm_backward_operator();
+  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor>(
+      const Tensor&, const Tensor&, const Optional&, const Tensor&, const Tensor&, bool, bool, bool, int64_t)>(
+      "bilinear_hip::layer_norm_backward");
   const auto [dx, dw, db] = op.call(dy, x, given(w), moments.select(0, 0), moments.select(0, 1), need_x, need_weight,
                                     need_bias, code);
   return {wanted(need_x, dx), wanted(need_weight, dw), wanted(need_bias, db)};
@@ -314,17 +311,13 @@ std::tuple<Tensor, Tensor> custom_residual_norm(const Tensor& x, const Tensor& r
   return {std::get<0>(out), std::get<1>(out)};
 }
 
-auto residual_norm_backward_operator() {
-  return custom<std::tuple<Tensor, Tensor, Tensor, Tensor>(
-      const Tensor&, const Optional&, const Tensor&, const Optional&, const Tensor&, const Tensor&, double, c10::SymInt,
-      c10::SymInt, c10::SymInt, c10::SymInt, const Optional&, bool, bool, bool, bool, int64_t)>(
-      "bilinear_hip::residual_norm_backward");
-}
-
 variable_list custom_residual_norm_backward(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w,
                                             const Tensor& moments, const Draws& d, bool need_x, bool need_residual,
                                             bool need_weight, bool need_bias, int64_t code) {
-  static const auto op = residual_norm_backward_operator();
+  static const auto op = custom<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+      const Tensor&, const Optional&, const Tensor&, const Optional&, const Tensor&, const Tensor&, double, c10::SymInt,
+      c10::SymInt, c10::SymInt, c10::SymInt, const Optional&, bool, bool, bool, bool, int64_t)>(
+      "bilinear_hip::residual_norm_backward");
   const auto [dx, dres, dw, db] = op.call(dy, given(dh), h, given(w), moments.select(0, 0), moments.select(0, 1), d.p, d.seed,
                                           d.step, d.layer, d.row_offset, given(d.device_step), need_x, need_residual,
                                           need_weight, need_bias, code);
@@ -384,35 +377,22 @@ bool any_needs_grad(std::initializer_list<const Tensor*> inputs) {
   return false;
 }
 
-// The custom backward operators under autograd: the same refusals.  (In C++: as a Python formula they cost 3 us a call.)
-std::tuple<Tensor, Tensor, Tensor> autograd_layer_norm_backward(c10::DispatchKeySet keys, const Tensor& dy,
-                                                                const Tensor& x, const Optional& weight, const Tensor& mean,
-                                                                const Tensor& rstd, bool need_x, bool need_weight,
-                                                                bool need_bias, int64_t code) {
-  static const auto op = layer_norm_backward_operator();
-  const Tensor w = plain(weight);
-  refuse_tangents({&dy, &x, &w, &mean, &rstd});
-  const bool refuse = any_needs_grad({&dy, &x, &w, &mean, &rstd});
-  auto out = op.redispatch(keys & c10::after_autograd_keyset, dy, x, weight, mean, rstd, need_x, need_weight, need_bias, code);
-  if (!refuse) return out;
-  const variable_list g = once({std::get<0>(out), std::get<1>(out), std::get<2>(out)});
-  return {g[0], g[1], g[2]};
-}
-
-std::tuple<Tensor, Tensor, Tensor, Tensor> autograd_residual_norm_backward(
-    c10::DispatchKeySet keys, const Tensor& dy, const Optional& dh, const Tensor& h, const Optional& weight,
-    const Tensor& mean, const Tensor& rstd, double p, c10::SymInt seed, c10::SymInt step, c10::SymInt layer,
-    c10::SymInt row_offset, const Optional& device_step, bool need_x, bool need_residual, bool need_weight, bool need_bias,
-    int64_t code) {
-  static const auto op = residual_norm_backward_operator();
-  const Tensor w = plain(weight), s = plain(dh);
-  refuse_tangents({&dy, &s, &h, &w, &mean, &rstd});
-  const bool refuse = any_needs_grad({&dy, &s, &h, &w, &mean, &rstd});
-  auto out = op.redispatch(keys & c10::after_autograd_keyset, dy, dh, h, weight, mean, rstd, p, seed, step, layer, row_offset,
-                           device_step, need_x, need_residual, need_weight, need_bias, code);
-  if (!refuse) return out;
-  const variable_list g = once({std::get<0>(out), std::get<1>(out), std::get<2>(out), std::get<3>(out)});
-  return {g[0], g[1], g[2], g[3]};
+// The custom backward operators under autograd: the same refusals.  (As a Python formula they cost 3 us a call.)
+void autograd_of_backward(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  bool refuse = false;
+  for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size())) {
+    if (!v.isTensor()) continue;
+    const Tensor& t = v.toTensor();
+    refuse_tangents({&t});
+    refuse = refuse || any_needs_grad({&t});
+  }
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+  if (!refuse || !at::GradMode::is_enabled()) return;
+  const size_t n = op.schema().returns().size();
+  variable_list out;
+  for (const c10::IValue& v : torch::jit::last(*stack, n)) out.push_back(v.toTensor());
+  torch::jit::drop(*stack, n);
+  for (Tensor& t : once(std::move(out))) torch::jit::push(*stack, std::move(t));
 }
 
 struct LayerNormBackward : public torch::autograd::Node {
@@ -669,8 +649,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_residual_norm_backward(
 }  // namespace
 
 TORCH_LIBRARY_IMPL(bilinear_hip, AutogradCUDA, m) {
-  m.impl("layer_norm_backward", &autograd_layer_norm_backward);
-  m.impl("residual_norm_backward", &autograd_residual_norm_backward);
+  m.impl("layer_norm_backward", torch::CppFunction::makeFromBoxedFunction<&autograd_of_backward>());
+  m.impl("residual_norm_backward", torch::CppFunction::makeFromBoxedFunction<&autograd_of_backward>());
 }
 
 PYBIND11_MODULE(_rows, m) {
