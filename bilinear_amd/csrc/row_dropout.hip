@@ -9,8 +9,8 @@
 // over devices.  p is rounded to a multiple of 2^-16 and s is the exact inverse of the rounded keep probability, so the
 // expectation of y is x.  The backward pass is the same map on dy: there is nothing to save.
 //
-// Bound by memory: 16384 x 2048 bf16 22.6 us = 5.9 TB/s of its bytes on three inputs in turn, 27 us = 5.0 where forward and
-// backward alternate on 800 MB (a copy of 537 MB: 5.0); a stored mask of one bit would add 3 % to a 16-bit type's bytes
+// Bound by memory: 16384 x 2048 bf16 22.4 us = 6.0 TB/s of its bytes over and over on three inputs in turn (a copy in the same
+// loop 19.5), 25 us = 5.3 among the other operators on 800 MB (a copy of 537 MB: 5.4); a stored mask of one bit would add 3 % to a 16-bit type's bytes
 // each way.  A draw takes 16 bits so that a call, 20 multiplies, serves 8 elements.
 #include "row_ops.h"
 #include "row_ops_dev.h"

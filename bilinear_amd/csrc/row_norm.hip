@@ -215,9 +215,10 @@ __global__ __launch_bounds__(1024) void norm_bwd_finish_kernel(NormBwd p) {
 
 // ---- rows that stay in registers --------------------------------------------------------------------------------------
 // LANES lanes own a row, NV units each: one read of every input, one write of every output, so what bounds these kernels is
-// memory (16384 x 2048, all tensors in turn, bf16 on an fp32 stream where there is one: layer norm forward 22.8 us = 5.9 TB/s
-// of its bytes, backward with its finish 38.7 us = 5.2 TB/s, residual norm 75.7 us = 5.3 and 102 us = 5.2 TB/s; a copy of
-// such tensors reaches 5.0-5.3).  Up to 64 lanes a row needs no barrier; a longer one joins its waves' sums through LDS, two
+// memory (16384 x 2048 bf16, one operation over and over on three inputs in turn: layer norm forward 22.9 us, backward with its
+// finish 39 us, on an fp32 stream residual norm 76 and 104 us; a copy of as many bytes in the same loop 19.5, 35, 74 and 100).
+// One kernel does not fit: the residual norm's backward of 8193 to 16384 columns on an fp32 stream spills 10 to 14 registers
+// a lane (1024 x 16384 fp32 96 us = 3.5 TB/s of its bytes).  Up to 64 lanes a row needs no barrier; a longer one joins its waves' sums through LDS, two
 // buffers in turn (one barrier per sum).
 
 template <int LANES> struct RowGroup {
@@ -509,8 +510,8 @@ static constexpr int64_t ROW_RESIDENT = 16384;     // widest row that stays in r
 // against 72.8; 1024 blocks of 256 threads 73).
 static constexpr int64_t ROW_TWO_BLOCKS = 1024;
 static int norm_blocks(int64_t width) { return width <= ROW_TWO_BLOCKS ? 512 : 256; }
-// One launch without partial sums (norm_few_cols) for few rows.  Kernel time, first launch's start to last one's end, of 64 /
-// 512 / 1024 / 2048 rows of 1024 bf16: 4.3 / 6.3 / 9.1 / 14.1 us, by the two launches 15.8 / 16.3 / 15.1 / 15.2 (2048
+// One launch without partial sums (norm_few_cols) for few rows.  Kernel time, first launch's start to last one's end, on the
+// same tensors again and again (on others in turn 12.5 us for 1024 rows of 1024), of 64 / 512 / 1024 / 2048 rows of 1024 bf16: 4.3 / 6.3 / 9.1 / 14.1 us, by the two launches 15.8 / 16.3 / 15.1 / 15.2 (2048
 // columns: 4.3 / 6.8 / 10.0 / 22.8 against 15.9 / 15.3 / 16.8 / 16.4).
 static bool norm_few(int64_t rows, int64_t width) { return rows > 0 && rows <= 1024 && width <= 4096; }
 static int norm_partials(int64_t rows, int64_t width) {

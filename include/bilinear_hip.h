@@ -44,7 +44,8 @@ extern "C" {
  * small-batch launches) were removed with the slower opt-in variants they served.
  * 6 (round 6): blh_comm_* / blh_rccl_* / blh_train_step_dp (collectives issued by the library) and BLH_ERR_COMM added;
  * nothing removed or changed.  (The row operators — blh_layer_norm_*, blh_residual_norm_*, blh_row_* — came later
- * under the same number: new names only, what version 6 had is as it was.)                                  */
+ * under the same number: new names only, what version 6 had is as it was.  Who loads the library at run time finds out by
+ * looking a name up, e.g. blh_row_dropout.)                                                                  */
 #define BLH_ABI_VERSION 6
 
 typedef enum {
@@ -494,7 +495,7 @@ int blh_heavy_backward(blh_context* ctx, void* stream, const float* d_out, const
  * element i * ld (ld >= 0: rows of a wider tensor, or one row repeated with ld = 0), outputs dense.  Base pointers are
  * aligned to their element only; any width from 1 to 2^24, any number of rows (0: nothing is read, weight gradients are
  * zero).  Types: activations `dtype`; `param_dtype` (weight, bias and their gradients) and `stream_dtype` (the residual
- * stream) are `dtype` or BLH_F32.  Sums, means and moments are fp32; every result is rounded once.  No atomics: results
+ * stream) are `dtype` or BLH_F32.  All arithmetic is fp32; a 16-bit result is its fp32 value, rounded once.  No atomics: results
  * do not change from run to run.  Inputs and outputs must not overlap, except that blh_row_dropout may work in place
  * (y == x, ldx == width).  A row that holds an infinity or NaN makes that row's results NaN and no other's.           */
 typedef enum { BLH_F32 = 0, BLH_BF16 = 1, BLH_F16 = 2 } blh_dtype;
