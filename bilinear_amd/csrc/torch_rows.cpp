@@ -15,7 +15,6 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
@@ -352,18 +351,8 @@ template <typename L> void refuse_eager_leaves(const L& inputs) {
   }
 }
 
-// The norms' formulas below are not themselves differentiable: under create_graph their results refuse a backward pass through
-// them.  (The error's node is attached to tensors that need a gradient alone, which fresh results do not.)
-variable_list once(variable_list grads) {
-  if (!at::GradMode::is_enabled()) return grads;
-  for (Tensor& g : grads) {
-    if (!g.defined()) continue;
-    g = g.detach();
-    g.set_requires_grad(true);
-  }
-  const auto error = std::make_shared<torch::autograd::DelayedError>(
-      "bilinear_amd row operators: trying to differentiate the backward pass, which is not supported", (int64_t)grads.size());
-  return (*error)(std::move(grads));
+template <typename N> std::shared_ptr<N> make_node() {
+  return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
 }
 
 void refuse_tangents(std::initializer_list<const Tensor*> inputs) {
@@ -378,22 +367,43 @@ bool any_needs_grad(std::initializer_list<const Tensor*> inputs) {
   return false;
 }
 
+// The norms' formulas below are not themselves differentiable.  Under create_graph their results belong to a node that leads
+// on to what they depend on and refuses to run: whoever differentiates them, towards whichever input, meets it.  (torch's own
+// DelayedError leads nowhere: torch.autograd.grad would pass it by and leave the term out.)
+struct SecondDerivative : public torch::autograd::Node {
+  std::string name() const override { return "BilinearSecondDerivative"; }
+  variable_list apply(variable_list&&) override {
+    TORCH_CHECK(false, "bilinear_amd row operators: trying to differentiate the backward pass, which is not supported");
+  }
+};
+
+variable_list once(variable_list grads, const variable_list& inputs) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::edge_list edges;
+  for (const Tensor& t : inputs)
+    if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+  if (edges.empty()) return grads;
+  const auto node = make_node<SecondDerivative>();
+  node->set_next_edges(std::move(edges));
+  for (const Tensor& g : grads)
+    if (g.defined()) torch::autograd::set_history(g, node);
+  return grads;
+}
+
 // The custom backward operators under autograd: the same refusals.  (As a Python formula they cost 3 us a call.)
 void autograd_of_backward(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
-  bool refuse = false;
+  variable_list inputs;
   for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size())) {
     if (!v.isTensor()) continue;
     const Tensor& t = v.toTensor();
     refuse_tangents({&t});
-    refuse = refuse || any_needs_grad({&t});
+    if (t.requires_grad()) inputs.push_back(t);
   }
   op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
-  if (!refuse || !at::GradMode::is_enabled()) return;
-  const size_t n = op.schema().returns().size();
+  if (inputs.empty() || !at::GradMode::is_enabled()) return;
   variable_list out;
-  for (const c10::IValue& v : torch::jit::last(*stack, n)) out.push_back(v.toTensor());
-  torch::jit::drop(*stack, n);
-  for (Tensor& t : once(std::move(out))) torch::jit::push(*stack, std::move(t));
+  for (const c10::IValue& v : torch::jit::last(*stack, op.schema().returns().size())) out.push_back(v.toTensor());
+  once(std::move(out), inputs);
 }
 
 struct LayerNormBackward : public torch::autograd::Node {
@@ -415,7 +425,8 @@ struct LayerNormBackward : public torch::autograd::Node {
                need_b = task_should_compute_output(2);
     if (followed({&grads[0], &in, &w}))
       return custom_layer_norm_backward(grads[0], in, w, moments, need_x, need_w, need_b, code);
-    return once(layer_norm_backward_launch(grads[0], in, dense(w), Moments(moments), need_x, need_w, need_b, code));
+    return once(layer_norm_backward_launch(grads[0], in, dense(w), Moments(moments), need_x, need_w, need_b, code),
+                {grads[0], in, w});
   }
 };
 
@@ -467,17 +478,13 @@ struct ResidualNormBackward : public torch::autograd::Node {
     if (followed({&dy, &grads[1], &stream, &w}))
       return custom_residual_norm_backward(dy, grads[1], stream, w, moments, d, need_x, need_r, need_w, need_b, code);
     // without dropout and with one type both branches of the sum get the same gradient: it is written once
-    const bool same = need_x && need_r && stream.scalar_type() == dtype && !drops;
+    const bool same = need_x && need_r && stream.scalar_type() == dtype && !drops && !at::GradMode::is_enabled();
     variable_list out = residual_norm_backward_launch(dy, grads[1], stream, dense(w), Moments(moments), d, need_x && !same,
                                                       need_r, need_w, need_b, code);
     if (same) out[0] = out[1];
-    return once(std::move(out));
+    return once(std::move(out), {dy, grads[1], stream, w});
   }
 };
-
-template <typename N> std::shared_ptr<N> make_node() {
-  return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
-}
 
 bool wants_grad(std::initializer_list<const Tensor*> inputs) {
   refuse_tangents(inputs);

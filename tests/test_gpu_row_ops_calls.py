@@ -40,6 +40,33 @@ def test_a_second_derivative_is_refused_beside_other_terms(B, name):
         (y.sum() + g.square().sum()).backward()
 
 
+@pytest.mark.parametrize("name", ["layer_norm", "residual_norm", "residual_norm without dropout", "operator layer_norm",
+                                  "operator residual_norm"])
+def test_a_second_derivative_is_refused_towards_chosen_inputs(B, name):
+    """torch.autograd.grad runs what leads to the inputs it is given, and functional.hessian takes what does not for zero."""
+    def tensors():
+        x, r = data(3, 16, F32, 1).requires_grad_(), data(3, 16, F32, 2).requires_grad_()
+        return (x, r, *params(16, F32, 5))
+    f = _first_outputs(B)[name]
+    for of in (0, 2):                                       # of dx, of dweight
+        for towards in (0, 2):
+            args = tensors()
+            y = f(*args)
+            g, = torch.autograd.grad(y.square().sum(), args[of], create_graph=True)
+            with pytest.raises(RuntimeError, match="differentiate the backward pass"):
+                torch.autograd.grad(y.sum() + g.square().sum(), args[towards], allow_unused=True)
+    x, r, w, b = tensors()
+    with pytest.raises(RuntimeError, match="differentiate the backward pass"):
+        torch.autograd.functional.hessian(lambda t: f(t, r, w, b).pow(3).sum(), x.detach())
+
+
+def test_a_graph_of_gradients_that_depend_on_nothing_more_is_plain(B):
+    x = data(3, 16, F32, 1)
+    w, b = params(16, F32, 5)
+    db, = torch.autograd.grad(B.layer_norm(x, w.detach(), b).sum(), b, create_graph=True)
+    assert not db.requires_grad
+
+
 def test_the_backward_operators_refuse_to_be_differentiated(B):
     op = torch.ops.bilinear_hip
     x, dy = data(3, 16, F32, 1), data(3, 16, F32, 2).requires_grad_()
