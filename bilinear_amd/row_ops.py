@@ -205,10 +205,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def dropout(x, p, seed, step=0, layer=0, row_offset=0, device_step=None):
     """Drop elements of ``x`` with probability ``p`` (rounded to a multiple of 2^-16) and scale the others so that the
     expectation stays; what is dropped is zero whatever it held.  The mask depends on (seed, step, layer, global row,
-    column) alone — one word of the generator's key is ``seed ^ (step >> 32)``, so let steps that count stay below 2^32 where
-    several seeds are in use — ``row_offset`` is the global index of the first row, so a batch split over devices draws the mask of
-    the whole one — and is drawn again in the backward pass instead of being stored.  ``device_step``: an int64 tensor
-    that is added to ``step`` when the kernel runs: a captured graph that advances it draws another mask each replay."""
+    column) alone — ``row_offset`` is the global index of the first row, so a batch split over devices draws the mask of
+    the whole one — and is drawn again in the backward pass instead of being stored.  One word of the generator's key is
+    ``seed ^ (step >> 32)``: let steps that count stay below 2^32 where several seeds are in use.  ``device_step``: an
+    int64 tensor that is added to ``step`` when the kernel runs: a captured graph that advances it draws another mask each
+    replay."""
     if torch.compiler.is_compiling():
         return torch.ops.bilinear_hip.row_dropout(x, p, seed, step, layer, row_offset, device_step)[0]
     return (_rows or _native()).dropout(x, p, seed, step, layer, row_offset, device_step)

@@ -404,3 +404,15 @@ def test_tensors_whose_storage_is_gone_are_refused(B):
                  lambda: torch.ops.bilinear_hip.layer_norm(x, gone, None, 1e-5)):
         with pytest.raises(RuntimeError, match="no storage"):
             call()
+
+
+def test_wrappers_of_function_transforms_are_refused(B):
+    """None of them is taken for a parameter that was left out."""
+    x, w = data(4, 16, F32, 1).contiguous(), params(16, F32, 5)[0].detach()
+    for call in (lambda: torch.func.functionalize(lambda t: B.layer_norm(x, t))(w),
+                 lambda: torch.func.functionalize(lambda t: B.residual_norm(x, x, None, t)[0])(w),
+                 lambda: torch.func.grad(lambda t: B.layer_norm(x, t).sum())(w),
+                 lambda: torch.vmap(lambda t: B.layer_norm(x, t))(w.expand(2, 16)),
+                 lambda: torch.func.jvp(lambda t: B.layer_norm(x, t), (w,), (w,))):
+        with pytest.raises(RuntimeError):
+            call()
